@@ -365,6 +365,112 @@ float *qdb_mel_spectrogram(const float *samples, int n_samples, int *out_frames)
  * cudaStream_t as void*, NULL = the legacy default stream). 0 = ok. */
 int qdb_mel_spectrogram_device(const float *samples_dev, int n_samples, float *mel_dev, void *stream);
 
+/* ---- Operators on a paged KV cache, and sampling. No counterpart in the
+ * reference, whose cache is one growing array per utterance and whose decoding
+ * is greedy.
+ *
+ * Like qdb_mel_spectrogram_device they take DEVICE pointers, run on the
+ * current CUDA device and are enqueued on `stream` (a cudaStream_t as void*,
+ * NULL = the legacy default stream); they allocate nothing, do not
+ * synchronise and may be captured into a graph. A host pointer, or one of
+ * another device, is refused. Head dimension 128. 0 = ok, -1 = error. ---- */
+enum { QDB_TYPE_F32 = 0, QDB_TYPE_F16 = 1, QDB_TYPE_BF16 = 2 };
+
+/* One layer's keys and values in pages of page_size positions (16, 32, 64, 128
+ * or 256). Element (page p, head g, slot s, dim d) of either pool is at
+ * p * page_stride + g * head_stride + s * pos_stride + d elements; all strides
+ * 0 = contiguous [page][head][slot][128]. Strides are multiples of 8 elements,
+ * the pools start on 16-byte boundaries. type: QDB_TYPE_F16 or QDB_TYPE_BF16. */
+typedef struct {
+    void *k, *v;
+    int type;
+    int n_pages, page_size, kv_heads;
+    long long page_stride, head_stride, pos_stride;
+} qdb_paged_kv;
+
+/* The sequences of one call. Sequence b owns rows q_starts[b] ..
+ * q_starts[b + 1] - 1 (device int [n_seqs + 1]; NULL: row b is sequence b, and
+ * rows = n_seqs); they are its newest positions, so its row i of n is at
+ * position kv_lens[b] - n + i. kv_lens (device int [n_seqs]) counts the new
+ * rows; its position p is on page tables[b * table_stride + p / page_size].
+ * Rows from q_starts[n_seqs] up to `rows` belong to no sequence: what they
+ * hold is not read and their outputs are left as they were. Table entries
+ * behind a sequence's length are not read.
+ * err (nullable, device int [4], zeroed by the caller): a page id outside the
+ * pool, a position behind the page table or the rotation table, or a row range
+ * outside [0, rows] is never accessed, and the first one is recorded here as
+ * {3, check, sequence, value}; the outputs of such a sequence are unspecified. */
+typedef struct {
+    int n_seqs, rows;
+    const int *q_starts;
+    const int *kv_lens;
+    const int *tables;
+    int table_stride;
+    int *err;
+} qdb_paged_batch;
+
+/* Takes rows of the QKV projection [rows, (heads + 2 kv_heads) * 128] (query
+ * heads, then key heads, then value heads; src_type f32, f16 or bf16), applies
+ * the per-head RMSNorm to queries and keys (q_norm / k_norm f32 [128], either
+ * NULL = none) and the rotation of each head's halves by the row's position
+ * (rope: f32 [rope_len][64][2] = cos, sin; NULL = none), writes keys and
+ * values into the cache and the queries to q_out [rows, heads * 128] in the
+ * cache's type. f16 stores saturate at +-65504. row_stride / q_stride: elements
+ * between rows (0 = contiguous), multiples of 16 bytes. A row at a negative
+ * position (more rows than kv_lens) is left out. Up to 16 query heads per key
+ * head. A position must not occur twice in one call. */
+int qdb_paged_append(const qdb_paged_kv *kv, const qdb_paged_batch *batch, const void *qkv, int src_type,
+                     long long row_stride, int heads, const float *q_norm, const float *k_norm, float eps,
+                     const float *rope, int rope_len, void *q_out, long long q_stride, void *stream);
+
+/* Scratch of qdb_paged_decode on `device` (about 3 MB, allocated and cleared
+ * here). One call uses it at a time: calls that may overlap on the GPU (two
+ * streams, two graphs replayed at once) need one each. NULL on error. */
+typedef struct qdb_paged_workspace qdb_paged_workspace;
+qdb_paged_workspace *qdb_paged_workspace_create(int device);
+void qdb_paged_workspace_free(qdb_paged_workspace *ws);
+
+/* Attention of one new row per sequence (batch->q_starts NULL) over its
+ * kv_lens[b] cached positions: out = softmax(scale * q K^T) V. q and out
+ * [rows, heads * 128] in the cache's type, q_stride / out_stride elements
+ * between rows (0 = contiguous, multiples of 8); scale 0 = 1/sqrt(128). Query
+ * head h reads key head h / (heads / kv_heads); at most 16 query heads per key
+ * head. A sequence of length 0 gives a row of zeros. */
+int qdb_paged_decode(const qdb_paged_kv *kv, const qdb_paged_batch *batch, const void *q, long long q_stride,
+                     int heads, float scale, void *out, long long out_stride, qdb_paged_workspace *ws, void *stream);
+
+/* Causal attention of each sequence's new rows over its cached positions, the
+ * new ones among them: the row at position p sees positions 0 .. p. Arguments
+ * as for qdb_paged_decode; a row at a negative position gives zeros. */
+int qdb_paged_prompt(const qdb_paged_kv *kv, const qdb_paged_batch *batch, const void *q, long long q_stride,
+                     int heads, float scale, void *out, long long out_stride, void *stream);
+
+/* Per-row sampling parameters (device arrays [rows]; NULL = the value in
+ * brackets): temperature [1] (not above 0: greedy, lowest index first), top_k
+ * [0 = off], top_p [1 = off], min_p [0 = off], and one random number in [0, 1)
+ * per row (required). */
+typedef struct {
+    const float *temperature;
+    const int *top_k;
+    const float *top_p;
+    const float *min_p;
+    const float *uniform;
+} qdb_sampling;
+
+#define QDB_SAMPLE_MAX_VOCAB 262144
+
+/* One token per row of logits [rows, vocab] (f32, f16 or bf16; row_stride
+ * elements, 0 = vocab). With w_i = exp((l_i - max) / temperature) and tokens
+ * ordered by logit, ties by index, a token stays if its rank is below top_k,
+ * the weights before it sum to less than top_p of the top_k's, and w_i >=
+ * min_p (the first token always stays). The result is the first token that
+ * stays, in index order, at which the running sum of the weights exceeds
+ * uniform * total. Sums are exact integers in units of 2^-45 of the largest
+ * weight: the result does not depend on the run. NaN and -inf logits are never
+ * drawn; a row with nothing else gives -1. */
+int qdb_sample(const void *logits, int type, long long row_stride, int rows, int vocab, const qdb_sampling *s,
+               int *tokens_out, void *stream);
+
 /* Waits for all queued work of the model's stream. */
 int qdb_model_sync(qdb_model *m);
 

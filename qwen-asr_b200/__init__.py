@@ -38,6 +38,22 @@ class QdbConfig(ctypes.Structure):
                 ("vocab", ctypes.c_int), ("eps", ctypes.c_float), ("theta", ctypes.c_float)]
 
 
+class QdbPagedKV(ctypes.Structure):
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("type", ctypes.c_int), ("n_pages", ctypes.c_int),
+                ("page_size", ctypes.c_int), ("kv_heads", ctypes.c_int), ("page_stride", ctypes.c_longlong),
+                ("head_stride", ctypes.c_longlong), ("pos_stride", ctypes.c_longlong)]
+
+
+class QdbPagedBatch(ctypes.Structure):
+    _fields_ = [("n_seqs", ctypes.c_int), ("rows", ctypes.c_int), ("q_starts", ctypes.c_void_p),
+                ("kv_lens", ctypes.c_void_p), ("tables", ctypes.c_void_p), ("table_stride", ctypes.c_int),
+                ("err", ctypes.c_void_p)]
+
+
+class QdbSampling(ctypes.Structure):
+    _fields_ = [(k, ctypes.c_void_p) for k in ("temperature", "top_k", "top_p", "min_p", "uniform")]
+
+
 # Every symbol include/qwen_asr_b200.h declares: name -> (restype, argtypes).
 ABI = {
     "qdb_last_error": (ctypes.c_char_p, []),
@@ -92,6 +108,20 @@ ABI = {
     "qdb_forward_noalloc": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p]),
     "qdb_model_stream": (ctypes.c_void_p, [ctypes.c_void_p]),
     "qdb_model_set_wait_limit": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_longlong]),
+    "qdb_paged_append": (ctypes.c_int, [ctypes.POINTER(QdbPagedKV), ctypes.POINTER(QdbPagedBatch), ctypes.c_void_p,
+                                        ctypes.c_int, ctypes.c_longlong, ctypes.c_int, ctypes.c_void_p,
+                                        ctypes.c_void_p, ctypes.c_float, ctypes.c_void_p, ctypes.c_int,
+                                        ctypes.c_void_p, ctypes.c_longlong, ctypes.c_void_p]),
+    "qdb_paged_workspace_create": (ctypes.c_void_p, [ctypes.c_int]),
+    "qdb_paged_workspace_free": (None, [ctypes.c_void_p]),
+    "qdb_paged_decode": (ctypes.c_int, [ctypes.POINTER(QdbPagedKV), ctypes.POINTER(QdbPagedBatch), ctypes.c_void_p,
+                                        ctypes.c_longlong, ctypes.c_int, ctypes.c_float, ctypes.c_void_p,
+                                        ctypes.c_longlong, ctypes.c_void_p, ctypes.c_void_p]),
+    "qdb_paged_prompt": (ctypes.c_int, [ctypes.POINTER(QdbPagedKV), ctypes.POINTER(QdbPagedBatch), ctypes.c_void_p,
+                                        ctypes.c_longlong, ctypes.c_int, ctypes.c_float, ctypes.c_void_p,
+                                        ctypes.c_longlong, ctypes.c_void_p]),
+    "qdb_sample": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_int, ctypes.c_int,
+                                  ctypes.POINTER(QdbSampling), ctypes.c_void_p, ctypes.c_void_p]),
     "qdb_trace_step": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int, ctypes.c_int,
                                       ctypes.POINTER(ctypes.c_uint64), ctypes.c_int]),
     "qdb_trace_batch_step": (ctypes.c_int, [ctypes.POINTER(ctypes.c_void_p), ctypes.c_int, _f32p, _i32p,
@@ -549,6 +579,99 @@ def mel_spectrogram_device(samples_ptr: int, n_samples: int, mel_ptr: int, strea
     if lib.qdb_mel_spectrogram_device(ctypes.c_void_p(samples_ptr), int(n_samples), ctypes.c_void_p(mel_ptr),
                                       ctypes.c_void_p(stream)):
         raise _err("qdb_mel_spectrogram_device")
+
+
+# ---- operators on a paged KV cache, and sampling (device pointers; see the header)
+TYPES = {"f32": 0, "f16": 1, "bf16": 2}
+
+
+def _type(name: str) -> int:
+    if name not in TYPES:
+        raise QdbError(f"type {name!r} is not one of {', '.join(TYPES)}")
+    return TYPES[name]
+
+
+class PagedKV:
+    """One layer's keys and values in pages: two device pools of n_pages pages of
+    page_size positions, dtype "f16" or "bf16", head dimension 128. layout "hnd" =
+    [page][head][slot][128], "nhd" = [page][slot][head][128]; strides = (page,
+    head, slot) in elements for any other order."""
+
+    def __init__(self, k: int, v: int, n_pages: int, page_size: int, kv_heads: int, dtype: str = "f16",
+                 layout: str = "hnd", strides=None):
+        if strides is None:
+            if layout == "hnd":
+                strides = (kv_heads * page_size * 128, page_size * 128, 128)
+            elif layout == "nhd":
+                strides = (kv_heads * page_size * 128, 128, kv_heads * 128)
+            else:
+                raise QdbError(f"layout {layout!r} is not hnd or nhd")
+        self.c = QdbPagedKV(k, v, _type(dtype), n_pages, page_size, kv_heads, *strides)
+
+
+class PagedBatch:
+    """The sequences of one call (device int arrays): n_seqs sequences with `rows`
+    new rows in all. q_starts [n_seqs + 1] (0: one row per sequence), kv_lens
+    [n_seqs] cached positions with the new ones, tables [n_seqs, table_stride]
+    page ids, err (0 or int [4]) the first refused access."""
+
+    def __init__(self, n_seqs: int, rows: int, kv_lens: int, tables: int, table_stride: int, q_starts: int = 0,
+                 err: int = 0):
+        self.c = QdbPagedBatch(n_seqs, rows, q_starts, kv_lens, tables, table_stride, err)
+
+
+class PagedWorkspace:
+    """Scratch of paged_decode on one device; one call uses it at a time."""
+
+    def __init__(self, device: int = 0):
+        self.h = lib.qdb_paged_workspace_create(device)
+        if not self.h:
+            raise _err("qdb_paged_workspace_create")
+
+    def close(self):
+        if self.h and not _exiting[0]:
+            lib.qdb_paged_workspace_free(self.h)
+        self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def paged_append(kv: PagedKV, batch: PagedBatch, qkv: int, q_out: int, heads: int, dtype: str = "f32",
+                 row_stride: int = 0, q_stride: int = 0, q_norm: int = 0, k_norm: int = 0, eps: float = 1e-6,
+                 rope: int = 0, rope_len: int = 0, stream: int = 0) -> None:
+    """Norms and rotates the queries and keys of QKV rows [rows, (heads + 2
+    kv_heads) * 128], writes keys and values into the cache and the queries to
+    q_out [rows, heads * 128] (the cache's type)."""
+    if lib.qdb_paged_append(kv.c, batch.c, qkv, _type(dtype), row_stride, heads, q_norm, k_norm, eps, rope, rope_len,
+                            q_out, q_stride, stream):
+        raise _err("qdb_paged_append")
+
+
+def paged_decode(kv: PagedKV, batch: PagedBatch, q: int, out: int, heads: int, workspace: PagedWorkspace,
+                 scale: float = 0.0, q_stride: int = 0, out_stride: int = 0, stream: int = 0) -> None:
+    """Attention of one new row per sequence over its cached positions."""
+    if lib.qdb_paged_decode(kv.c, batch.c, q, q_stride, heads, scale, out, out_stride, workspace.h, stream):
+        raise _err("qdb_paged_decode")
+
+
+def paged_prompt(kv: PagedKV, batch: PagedBatch, q: int, out: int, heads: int, scale: float = 0.0, q_stride: int = 0,
+                 out_stride: int = 0, stream: int = 0) -> None:
+    """Causal attention of each sequence's new rows over its cached positions."""
+    if lib.qdb_paged_prompt(kv.c, batch.c, q, q_stride, heads, scale, out, out_stride, stream):
+        raise _err("qdb_paged_prompt")
+
+
+def sample(logits: int, rows: int, vocab: int, uniform: int, tokens: int, dtype: str = "f32", row_stride: int = 0,
+           temperature: int = 0, top_k: int = 0, top_p: int = 0, min_p: int = 0, stream: int = 0) -> None:
+    """One token per row of logits, drawn with the given random numbers; the
+    parameters are device arrays [rows] (0 = off; see qdb_sample)."""
+    s = QdbSampling(temperature, top_k, top_p, min_p, uniform)
+    if lib.qdb_sample(logits, _type(dtype), row_stride, rows, vocab, s, tokens, stream):
+        raise _err("qdb_sample")
 
 
 def decode_greedy_batch(sessions, first_tokens, pos, n_steps: int) -> np.ndarray:

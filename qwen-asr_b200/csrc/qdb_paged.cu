@@ -1,0 +1,395 @@
+// qdb_paged.cu - paged KV cache: rotation and append of new positions, and
+// attention over the pages.
+#include <math.h>
+#include <stdio.h>
+
+#include "qdb_kernels.h"
+#include "qdb_paged.cuh"
+
+namespace {
+
+// ---------------------------------------------------------------- append
+// y = x * rsqrt(mean(x^2) + eps) * w for query and key heads (where norms are
+// given), then the rotation of the halves (a, b) -> (a c - b s, b c + a s)
+// with (c, s) the position's table row; values as they are.
+
+// Sequence of a row: the last b with q_starts[b] <= row (rows behind the last
+// sequence: n_seqs).
+__device__ __forceinline__ int row_sequence(const QdbPagedBatch &bt, int row) {
+    if (!bt.q_starts) return row;
+    int lo = 0, hi = bt.n_seqs;  // q_starts[lo] <= row < q_starts[hi + 1] as far as known
+    if (bt.q_starts[hi] <= row) return bt.n_seqs;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (bt.q_starts[mid] <= row) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+template <typename S>
+__device__ __forceinline__ float load_src(const void *p, size_t i);
+struct SrcF32 {};
+template <>
+__device__ __forceinline__ float load_src<SrcF32>(const void *p, size_t i) {
+    return reinterpret_cast<const float *>(p)[i];
+}
+template <>
+__device__ __forceinline__ float load_src<QdbHalf>(const void *p, size_t i) {
+    return QdbHalf::lo(reinterpret_cast<const uint16_t *>(p)[i]);
+}
+template <>
+__device__ __forceinline__ float load_src<QdbBf16>(const void *p, size_t i) {
+    return QdbBf16::lo(reinterpret_cast<const uint16_t *>(p)[i]);
+}
+
+// One warp per (row, head vector).
+template <typename S, typename T>
+__global__ void append_kernel(const QdbAppendArgs a) {
+    pdl_enter();
+    const int lane = threadIdx.x & 31;
+    const int slot = blockIdx.y * (blockDim.x >> 5) + (threadIdx.x >> 5);
+    const int row = blockIdx.x, Hq = a.heads, Hkv = a.kv.kv_heads;
+    if (slot >= Hq + 2 * Hkv) return;
+    const int b = row_sequence(a.bt, row);
+    if (b >= a.bt.n_seqs) return;
+    int first, last;
+    paged_rows(a.bt, b, first, last);
+    if (row < first || row >= last) return;
+    const int len = paged_len(a.bt, b, a.kv.page_shift, a.bt.step ? *a.bt.step : 0);
+    const int pos = len - (last - row);
+    if (pos < 0) return;  // the sequence is shorter than its rows
+    // a row that cannot be rotated is left out whole
+    if (a.rope && !check_or_record(pos < a.rope_len, a.bt.err, QDB_CHECK_ROPE, b, pos)) return;
+    float e[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) e[i] = load_src<S>(a.qkv, (size_t)row * a.row_stride + slot * QDB_HD + lane + 32 * i);
+    if (slot < Hq + Hkv) {
+        const float *w = slot < Hq ? a.q_norm : a.k_norm;
+        if (w) {
+            const float ss = warp_sum(e[0] * e[0] + e[1] * e[1] + e[2] * e[2] + e[3] * e[3]);
+            const float inv = 1.0f / sqrtf(ss / (float)QDB_HD + a.eps);
+#pragma unroll
+            for (int i = 0; i < 4; i++) e[i] = e[i] * inv * w[lane + 32 * i];
+        }
+        if (a.rope) {
+            const float2 *rr = a.rope + (size_t)pos * (QDB_HD / 2);
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const float2 cs = rr[lane + 32 * i];
+                const float x1 = e[i], x2 = e[i + 2];
+                e[i] = x1 * cs.x - x2 * cs.y;
+                e[i + 2] = x2 * cs.x + x1 * cs.y;
+            }
+        }
+    }
+    uint16_t *dst;
+    if (slot < Hq) {
+        dst = a.q_out + (size_t)row * a.q_stride + (size_t)slot * QDB_HD;
+    } else {
+        const int page = paged_page(a.kv, a.bt, b, pos >> a.kv.page_shift);
+        if (page < 0) return;
+        const bool is_k = slot < Hq + Hkv;
+        const int g = is_k ? slot - Hq : slot - Hq - Hkv;
+        dst = (is_k ? a.kv.k : a.kv.v) + page * a.kv.page_stride + g * a.kv.head_stride +
+              (pos & ((1 << a.kv.page_shift) - 1)) * a.kv.pos_stride;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) dst[lane + 32 * i] = T::one(e[i]);
+}
+
+// ---------------------------------------------------------------- attention
+// One warp per (row, query head), 32 keys at a time: lane j scores key j over
+// all 128 dims, then every lane sums 4 output dims over the 32 keys. Running
+// maximum and sum in f32.
+template <typename T>
+__global__ void attn_simple_kernel(const QdbPagedAttnArgs a) {
+    pdl_enter();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int row = blockIdx.x, head = blockIdx.y * (blockDim.x >> 5) + warp;
+    if (head >= a.heads) return;
+    const int b = row_sequence(a.bt, row);
+    if (b >= a.bt.n_seqs) return;
+    int first, last;
+    paged_rows(a.bt, b, first, last);
+    if (row < first || row >= last) return;
+    const int len = paged_len(a.bt, b, a.kv.page_shift, a.bt.step ? *a.bt.step : 0);
+    const int n = len - (last - 1 - row);  // keys this row sees
+    const int g = head / (a.heads / a.kv.kv_heads);
+    __shared__ __align__(16) float qs[8][QDB_HD];
+    const uint16_t *q = a.q + (size_t)row * a.q_stride + (size_t)head * QDB_HD;
+    for (int i = lane; i < QDB_HD; i += 32) qs[warp][i] = T::lo(q[i]) * a.scale;
+    __syncwarp();
+    float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int k0 = 0; k0 < n; k0 += 32) {
+        const int key = k0 + lane;
+        float s = -INFINITY;
+        long long at = -1;
+        if (key < n) {
+            const int page = paged_page(a.kv, a.bt, b, key >> a.kv.page_shift);
+            if (page >= 0) {
+                at = page * a.kv.page_stride + g * a.kv.head_stride +
+                     (key & ((1 << a.kv.page_shift) - 1)) * a.kv.pos_stride;
+                s = 0.f;
+                for (int d = 0; d < QDB_HD; d += 8) {
+                    const uint4 w = *reinterpret_cast<const uint4 *>(a.kv.k + at + d);
+                    const float *x = qs[warp] + d;
+                    s += T::lo(w.x) * x[0] + T::hi(w.x) * x[1] + T::lo(w.y) * x[2] + T::hi(w.y) * x[3] +
+                         T::lo(w.z) * x[4] + T::hi(w.z) * x[5] + T::lo(w.w) * x[6] + T::hi(w.w) * x[7];
+                }
+            }
+        }
+        const float mn = fmaxf(m, warp_max(s));
+        if (mn == -INFINITY) continue;
+        const float p = s == -INFINITY ? 0.f : expf(s - mn), f = m == -INFINITY ? 0.f : expf(m - mn);
+        m = mn;
+        l = l * f + warp_sum(p);
+#pragma unroll
+        for (int i = 0; i < 4; i++) o[i] *= f;
+        for (int j = 0; j < 32; j++) {
+            const long long aj = __shfl_sync(0xffffffffu, at, j);
+            const float pj = __shfl_sync(0xffffffffu, p, j);
+            if (aj < 0) continue;
+            const uint2 w = *reinterpret_cast<const uint2 *>(a.kv.v + aj + lane * 4);
+            o[0] += pj * T::lo(w.x);
+            o[1] += pj * T::hi(w.x);
+            o[2] += pj * T::lo(w.y);
+            o[3] += pj * T::hi(w.y);
+        }
+    }
+    const float inv = l > 0.f ? 1.0f / l : 0.f;
+    *reinterpret_cast<uint2 *>(a.out + (size_t)row * a.out_stride + (size_t)head * QDB_HD + lane * 4) =
+        make_uint2(T::pack(o[0] * inv, o[1] * inv), T::pack(o[2] * inv, o[3] * inv));
+}
+
+cudaError_t launch_simple(const QdbPagedAttnArgs &a, int type, cudaStream_t st) {
+    const dim3 grid(a.bt.rows, (a.heads + 7) / 8), block(256);
+    return type == QDB_TYPE_F16 ? pdl_launch(attn_simple_kernel<QdbHalf>, grid, block, 0, st, a)
+                                : pdl_launch(attn_simple_kernel<QdbBf16>, grid, block, 0, st, a);
+}
+
+}  // namespace
+
+cudaError_t qdb_launch_paged_append(const QdbAppendArgs &a, int src_type, int kv_type, cudaStream_t st) {
+    const int slots = a.heads + 2 * a.kv.kv_heads;
+    const dim3 grid(a.bt.rows, (slots + 7) / 8), block(256);
+    const bool h = kv_type == QDB_TYPE_F16;
+    if (src_type == QDB_TYPE_F32)
+        return h ? pdl_launch(append_kernel<SrcF32, QdbHalf>, grid, block, 0, st, a)
+                 : pdl_launch(append_kernel<SrcF32, QdbBf16>, grid, block, 0, st, a);
+    if (src_type == QDB_TYPE_F16)
+        return h ? pdl_launch(append_kernel<QdbHalf, QdbHalf>, grid, block, 0, st, a)
+                 : pdl_launch(append_kernel<QdbHalf, QdbBf16>, grid, block, 0, st, a);
+    return h ? pdl_launch(append_kernel<QdbBf16, QdbHalf>, grid, block, 0, st, a)
+             : pdl_launch(append_kernel<QdbBf16, QdbBf16>, grid, block, 0, st, a);
+}
+
+cudaError_t qdb_launch_paged_decode(const QdbPagedAttnArgs &a, int type, cudaStream_t st) {
+    return launch_simple(a, type, st);
+}
+cudaError_t qdb_launch_paged_prompt(const QdbPagedAttnArgs &a, int type, cudaStream_t st) {
+    return launch_simple(a, type, st);
+}
+
+// ---------------------------------------------------------------- C entry points
+// The device of a pointer is checked before every launch: a host pointer, or
+// one of another device than the current one, is refused instead of read.
+static bool on_device(const void *p, int dev, const char *what, char *msg, size_t len) {
+    cudaPointerAttributes at{};
+    const cudaError_t e = cudaPointerGetAttributes(&at, p);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        snprintf(msg, len, "%s: %s", what, cudaGetErrorString(e));
+        return false;
+    }
+    if (at.type != cudaMemoryTypeDevice && at.type != cudaMemoryTypeManaged) {
+        snprintf(msg, len, "%s is not a device pointer", what);
+        return false;
+    }
+    if (at.type == cudaMemoryTypeDevice && at.device != dev) {
+        snprintf(msg, len, "%s is on device %d, the current device is %d", what, at.device, dev);
+        return false;
+    }
+    return true;
+}
+
+int qdb_check_device_ptrs(const char *fn, const QdbNamedPtr *ps, int n) {
+    char msg[256], full[320];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        snprintf(full, sizeof(full), "%s: %s", fn, cudaGetErrorString(e));
+        return qdb_set_error(full);
+    }
+    for (int i = 0; i < n; i++)
+        if (ps[i].p && !on_device(ps[i].p, dev, ps[i].name, msg, sizeof(msg))) {
+            snprintf(full, sizeof(full), "%s: %s", fn, msg);
+            return qdb_set_error(full);
+        }
+    return 0;
+}
+
+#define REFUSE(cond, ...)                                     \
+    do {                                                      \
+        if (cond) {                                           \
+            char m_[320];                                     \
+            snprintf(m_, sizeof(m_), __VA_ARGS__);            \
+            return qdb_set_error(m_);                         \
+        }                                                     \
+    } while (0)
+
+static inline bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
+
+static int check_kv(const char *fn, const qdb_paged_kv *kv, QdbPagedKV *o) {
+    REFUSE(!kv || !kv->k || !kv->v, "%s: null cache", fn);
+    REFUSE(kv->type != QDB_TYPE_F16 && kv->type != QDB_TYPE_BF16, "%s: cache type %d is not f16 or bf16", fn, kv->type);
+    REFUSE(kv->n_pages <= 0 || kv->kv_heads <= 0, "%s: bad pool: %d pages of %d heads", fn, kv->n_pages, kv->kv_heads);
+    int shift = 4;
+    while (shift < 8 && (1 << shift) != kv->page_size) shift++;
+    REFUSE((1 << shift) != kv->page_size, "%s: page size %d is not 16, 32, 64, 128 or 256", fn, kv->page_size);
+    o->k = (uint16_t *)kv->k;
+    o->v = (uint16_t *)kv->v;
+    o->n_pages = kv->n_pages;
+    o->page_shift = shift;
+    o->kv_heads = kv->kv_heads;
+    o->page_stride = kv->page_stride;
+    o->head_stride = kv->head_stride;
+    o->pos_stride = kv->pos_stride;
+    if (!kv->page_stride && !kv->head_stride && !kv->pos_stride) {
+        o->pos_stride = QDB_HD;
+        o->head_stride = (long long)kv->page_size * QDB_HD;
+        o->page_stride = o->head_stride * kv->kv_heads;
+    }
+    const long long st[3] = {o->page_stride, o->head_stride, o->pos_stride};
+    for (long long s : st)
+        REFUSE(s < QDB_HD || s % 8 || s >= (1ll << 38), "%s: cache stride %lld (needs a multiple of 8 from 128 up)", fn, s);
+    REFUSE(!aligned16(kv->k) || !aligned16(kv->v), "%s: the cache must start on a 16-byte boundary", fn);
+    return 0;
+}
+
+static int check_batch(const char *fn, const qdb_paged_batch *b, QdbPagedBatch *o) {
+    REFUSE(!b, "%s: null batch", fn);
+    REFUSE(b->n_seqs < 0 || b->rows < 0, "%s: negative size", fn);
+    REFUSE(b->rows > (1 << 22), "%s: %d rows exceed the 4M-row limit", fn, b->rows);
+    REFUSE(b->n_seqs > (1 << 20), "%s: %d sequences exceed the 1M limit", fn, b->n_seqs);
+    *o = QdbPagedBatch{b->n_seqs, b->rows, b->q_starts, b->kv_lens, b->tables, b->table_stride, b->err, nullptr};
+    if (!b->n_seqs || !b->rows) return 0;
+    REFUSE(!b->kv_lens || !b->tables, "%s: null lengths or page tables", fn);
+    REFUSE(b->table_stride <= 0 || b->table_stride > (1 << 22), "%s: page tables of %d entries", fn, b->table_stride);
+    REFUSE(!b->q_starts && b->rows != b->n_seqs, "%s: %d rows of %d sequences need q_starts", fn, b->rows, b->n_seqs);
+    return 0;
+}
+
+static int check_heads(const char *fn, int heads, int kv_heads) {
+    REFUSE(heads <= 0 || heads % kv_heads || heads / kv_heads > 16 || heads > 1024,
+           "%s: %d heads over %d key heads (needs a multiple, at most 16 each)", fn, heads, kv_heads);
+    return 0;
+}
+
+static int launched(const char *fn, cudaError_t e) {
+    REFUSE(e != cudaSuccess, "%s: %s", fn, cudaGetErrorString(e));
+    return 0;
+}
+
+// Workspace of the one-token attention.
+struct qdb_paged_workspace {
+    int device;
+};
+
+extern "C" qdb_paged_workspace *qdb_paged_workspace_create(int device) {
+    qdb_set_error("");
+    const int n = qdb_device_count();
+    if (device < 0 || device >= n) {
+        char m[128];
+        snprintf(m, sizeof(m), "CUDA device %d not available (%d visible)", device, n);
+        qdb_set_error(m);
+        return nullptr;
+    }
+    return new qdb_paged_workspace{device};
+}
+
+extern "C" void qdb_paged_workspace_free(qdb_paged_workspace *ws) { delete ws; }
+
+extern "C" int qdb_paged_append(const qdb_paged_kv *kv, const qdb_paged_batch *batch, const void *qkv, int src_type,
+                                long long row_stride, int heads, const float *q_norm, const float *k_norm, float eps,
+                                const float *rope, int rope_len, void *q_out, long long q_stride, void *stream) {
+    const char *fn = "qdb_paged_append";
+    qdb_set_error("");
+    QdbAppendArgs a{};
+    if (check_kv(fn, kv, &a.kv) || check_batch(fn, batch, &a.bt) || check_heads(fn, heads, kv->kv_heads)) return -1;
+    REFUSE(src_type != QDB_TYPE_F32 && src_type != QDB_TYPE_F16 && src_type != QDB_TYPE_BF16, "%s: source type %d", fn,
+           src_type);
+    if (!a.bt.n_seqs || !a.bt.rows) return 0;
+    const long long width = (long long)(heads + 2 * kv->kv_heads) * QDB_HD;
+    const int unit = src_type == QDB_TYPE_F32 ? 4 : 8;
+    REFUSE(!qkv || !q_out, "%s: null rows", fn);
+    REFUSE((row_stride && row_stride < width) || row_stride % unit, "%s: row stride %lld", fn, row_stride);
+    REFUSE((q_stride && q_stride < (long long)heads * QDB_HD) || q_stride % 8, "%s: query stride %lld", fn, q_stride);
+    REFUSE(!aligned16(qkv) || !aligned16(q_out) || !aligned16(q_norm) || !aligned16(k_norm) || !aligned16(rope),
+           "%s: pointers must be on 16-byte boundaries", fn);
+    REFUSE(rope && rope_len <= 0, "%s: rotation table of %d positions", fn, rope_len);
+    const QdbNamedPtr ps[] = {{kv->k, "k"}, {kv->v, "v"}, {batch->q_starts, "q_starts"}, {batch->kv_lens, "kv_lens"},
+                           {batch->tables, "tables"}, {batch->err, "err"}, {qkv, "qkv"}, {q_norm, "q_norm"},
+                           {k_norm, "k_norm"}, {rope, "rope"}, {q_out, "q_out"}};
+    if (qdb_check_device_ptrs(fn, ps, (int)(sizeof(ps) / sizeof(ps[0])))) return -1;
+    a.qkv = qkv;
+    a.row_stride = row_stride ? row_stride : width;
+    a.heads = heads;
+    a.q_norm = q_norm;
+    a.k_norm = k_norm;
+    a.eps = eps;
+    a.rope = (const float2 *)rope;
+    a.rope_len = rope_len;
+    a.q_out = (uint16_t *)q_out;
+    a.q_stride = q_stride ? q_stride : (long long)heads * QDB_HD;
+    return launched(fn, qdb_launch_paged_append(a, src_type, kv->type, (cudaStream_t)stream));
+}
+
+// Checks of both attention forms; 1 = nothing to do.
+static int check_attn(const char *fn, const qdb_paged_kv *kv, const qdb_paged_batch *batch, const void *q,
+                      long long q_stride, int heads, float scale, void *out, long long out_stride,
+                      QdbPagedAttnArgs *a) {
+    if (check_kv(fn, kv, &a->kv) || check_batch(fn, batch, &a->bt) || check_heads(fn, heads, kv->kv_heads)) return -1;
+    REFUSE(!(scale >= 0.f) || scale > 3e38f, "%s: scale %g", fn, (double)scale);
+    if (!a->bt.n_seqs || !a->bt.rows) return 1;
+    const long long width = (long long)heads * QDB_HD;
+    REFUSE(!q || !out, "%s: null rows", fn);
+    REFUSE((q_stride && q_stride < width) || q_stride % 8, "%s: query stride %lld", fn, q_stride);
+    REFUSE((out_stride && out_stride < width) || out_stride % 8, "%s: output stride %lld", fn, out_stride);
+    REFUSE(!aligned16(q) || !aligned16(out), "%s: rows must start on 16-byte boundaries", fn);
+    const QdbNamedPtr ps[] = {{kv->k, "k"}, {kv->v, "v"}, {batch->q_starts, "q_starts"}, {batch->kv_lens, "kv_lens"},
+                           {batch->tables, "tables"}, {batch->err, "err"}, {q, "q"}, {out, "out"}};
+    if (qdb_check_device_ptrs(fn, ps, (int)(sizeof(ps) / sizeof(ps[0])))) return -1;
+    a->q = (const uint16_t *)q;
+    a->q_stride = q_stride ? q_stride : width;
+    a->heads = heads;
+    a->scale = scale > 0.f ? scale : 1.0f / sqrtf((float)QDB_HD);
+    a->out = (uint16_t *)out;
+    a->out_stride = out_stride ? out_stride : width;
+    return 0;
+}
+
+extern "C" int qdb_paged_decode(const qdb_paged_kv *kv, const qdb_paged_batch *batch, const void *q,
+                                long long q_stride, int heads, float scale, void *out, long long out_stride,
+                                qdb_paged_workspace *ws, void *stream) {
+    const char *fn = "qdb_paged_decode";
+    qdb_set_error("");
+    QdbPagedAttnArgs a{};
+    REFUSE(batch && batch->q_starts, "%s: one row per sequence (q_starts must be null)", fn);
+    REFUSE(!ws, "%s: null workspace", fn);
+    const int rc = check_attn(fn, kv, batch, q, q_stride, heads, scale, out, out_stride, &a);
+    if (rc) return rc < 0 ? -1 : 0;
+    return launched(fn, qdb_launch_paged_decode(a, kv->type, (cudaStream_t)stream));
+}
+
+extern "C" int qdb_paged_prompt(const qdb_paged_kv *kv, const qdb_paged_batch *batch, const void *q,
+                                long long q_stride, int heads, float scale, void *out, long long out_stride,
+                                void *stream) {
+    const char *fn = "qdb_paged_prompt";
+    qdb_set_error("");
+    QdbPagedAttnArgs a{};
+    const int rc = check_attn(fn, kv, batch, q, q_stride, heads, scale, out, out_stride, &a);
+    if (rc) return rc < 0 ? -1 : 0;
+    return launched(fn, qdb_launch_paged_prompt(a, kv->type, (cudaStream_t)stream));
+}

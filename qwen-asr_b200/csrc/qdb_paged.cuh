@@ -1,0 +1,141 @@
+// qdb_paged.cuh - the paged KV cache as the kernels see it: shared by the
+// append, the one-token attention and the prompt attention.
+//
+// One layer's keys and values lie in pages of `page` positions; a sequence's
+// positions [i * page, (i + 1) * page) are on page tables[b][i]. Element
+// (page p, head g, slot s, dim d) is at p * page_stride + g * head_stride +
+// s * pos_stride + d, so both [page][head][slot][128] and
+// [page][slot][head][128] pools are read in place.
+#pragma once
+#include <cuda_bf16.h>
+
+#include "../../include/qwen_asr_b200.h"
+#include "qdb_common.cuh"
+
+// Which check refused an access (err[1] of the caller's error words).
+enum {
+    QDB_CHECK_PAGE = 1,    // page id outside the pool: err[2] = sequence, err[3] = page id
+    QDB_CHECK_TABLE = 2,   // position behind the table's end: err[2] = sequence, err[3] = position
+    QDB_CHECK_ROPE = 3,    // position behind the rotation table: err[2] = sequence, err[3] = position
+    QDB_CHECK_STARTS = 4,  // row range outside [0, rows] or backwards: err[2] = sequence, err[3] = its end
+};
+
+struct QdbPagedKV {
+    uint16_t *k, *v;
+    int n_pages, page_shift, kv_heads;
+    long long page_stride, head_stride, pos_stride;
+};
+
+struct QdbPagedBatch {
+    int n_seqs, rows;
+    const int *q_starts;  // [n_seqs + 1], null: row b is sequence b
+    const int *lens;      // [n_seqs] positions, the new rows among them
+    const int *tables;    // [n_seqs][table_stride]
+    int table_stride;
+    int *err;         // nullable [4]
+    const int *step;  // nullable: added to every length (a captured step's counter)
+};
+
+// 16-bit element types of cache, queries and output.
+struct QdbHalf {
+    static constexpr int code = QDB_TYPE_F16;
+    static __device__ __forceinline__ float lo(uint32_t w) { return kvlo(w); }
+    static __device__ __forceinline__ float hi(uint32_t w) { return kvhi(w); }
+    // stores saturate at +-65504 (the cache's rule); NaN stays NaN
+    static __device__ __forceinline__ uint32_t pack(float a, float b) {
+        return (uint32_t)one(a) | ((uint32_t)one(b) << 16);
+    }
+    static __device__ __forceinline__ uint16_t one(float f) { return isnan(f) ? (uint16_t)0x7fffu : f32_to_kv(f); }
+};
+struct QdbBf16 {
+    static constexpr int code = QDB_TYPE_BF16;
+    static __device__ __forceinline__ float lo(uint32_t w) { return bf16lo(w); }
+    static __device__ __forceinline__ float hi(uint32_t w) { return bf16hi(w); }
+    static __device__ __forceinline__ uint32_t pack(float a, float b) {
+        const __nv_bfloat162 r = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&r);
+    }
+    static __device__ __forceinline__ uint16_t one(float f) { return f32_to_bf16_rn(f); }
+};
+
+// Length of sequence b: never negative, never behind its page table.
+__device__ __forceinline__ int paged_len(const QdbPagedBatch &bt, int b, int page_shift, int step) {
+    long long n = (long long)bt.lens[b] + step;
+    const long long most = (long long)bt.table_stride << page_shift;
+    if (n > most) {
+        check_or_record(false, bt.err, QDB_CHECK_TABLE, b, n);
+        n = most;
+    }
+    return n > 0 ? (int)n : 0;
+}
+
+// Rows [first, last) of sequence b, clamped to [0, rows] and never backwards.
+__device__ __forceinline__ void paged_rows(const QdbPagedBatch &bt, int b, int &first, int &last) {
+    if (!bt.q_starts) {
+        first = b;
+        last = b + 1;
+        return;
+    }
+    first = bt.q_starts[b];
+    last = bt.q_starts[b + 1];
+    if (first < 0 || last > bt.rows || last < first) {
+        check_or_record(false, bt.err, QDB_CHECK_STARTS, b, last);
+        first = last = 0;
+    }
+}
+
+// Page id of sequence b's i-th page, or -1 (recorded) when it is outside the pool.
+__device__ __forceinline__ int paged_page(const QdbPagedKV &kv, const QdbPagedBatch &bt, int b, int i) {
+    const int p = i < bt.table_stride ? bt.tables[(size_t)b * bt.table_stride + i] : -1;
+    return check_or_record(p >= 0 && p < kv.n_pages, bt.err, QDB_CHECK_PAGE, b, p) ? p : -1;
+}
+
+// ---- host checks: refuses host pointers and pointers of another device than
+// the current one (null pointers are left to the caller). 0 = ok.
+struct QdbNamedPtr {
+    const void *p;
+    const char *name;
+};
+int qdb_check_device_ptrs(const char *fn, const QdbNamedPtr *ps, int n);
+
+// ---- launchers (checked arguments) ----
+struct QdbAppendArgs {
+    QdbPagedKV kv;
+    QdbPagedBatch bt;
+    const void *qkv;
+    long long row_stride;  // elements of the source type
+    int heads;
+    const float *q_norm, *k_norm;  // nullable
+    float eps;
+    const float2 *rope;  // nullable
+    int rope_len;
+    uint16_t *q_out;
+    long long q_stride;
+};
+cudaError_t qdb_launch_paged_append(const QdbAppendArgs &a, int src_type, int kv_type, cudaStream_t st);
+
+struct QdbPagedAttnArgs {
+    QdbPagedKV kv;
+    QdbPagedBatch bt;
+    const uint16_t *q;
+    long long q_stride;
+    int heads;
+    float scale;
+    uint16_t *out;
+    long long out_stride;
+};
+cudaError_t qdb_launch_paged_decode(const QdbPagedAttnArgs &a, int type, cudaStream_t st);
+cudaError_t qdb_launch_paged_prompt(const QdbPagedAttnArgs &a, int type, cudaStream_t st);
+
+struct QdbSampleArgs {
+    const void *logits;
+    long long row_stride;
+    int rows, vocab;
+    const float *temperature;
+    const int *top_k;
+    const float *top_p, *min_p, *uniform;
+    int mask_eos;
+    int *tokens;
+    const int *step;  // nullable: uniform and tokens advance by *step * rows
+};
+cudaError_t qdb_launch_sample(const QdbSampleArgs &a, int type, cudaStream_t st);
