@@ -1,5 +1,7 @@
 // qdb_paged.cu - paged KV cache: rotation and append of new positions, and
 // attention over the pages.
+#include <cuda.h>
+#include <cudaTypedefs.h>
 #include <math.h>
 #include <stdio.h>
 
@@ -184,11 +186,38 @@ cudaError_t qdb_launch_paged_append(const QdbAppendArgs &a, int src_type, int kv
              : pdl_launch(append_kernel<QdbBf16, QdbBf16>, grid, block, 0, st, a);
 }
 
-cudaError_t qdb_launch_paged_decode(const QdbPagedAttnArgs &a, int type, cudaStream_t st) {
-    return launch_simple(a, type, st);
-}
 cudaError_t qdb_launch_paged_prompt(const QdbPagedAttnArgs &a, int type, cudaStream_t st) {
     return launch_simple(a, type, st);
+}
+
+cudaError_t qdb_decode_scratch_alloc(int device, QdbDecodeScratch *s) {
+    cudaError_t e = cudaDeviceGetAttribute(&s->ctas, cudaDevAttrMultiProcessorCount, device);
+    if (e == cudaSuccess) e = cudaMalloc((void **)&s->part, sizeof(float) * 2 * s->ctas * 16 * 130);
+    if (e == cudaSuccess) e = cudaMalloc((void **)&s->cnt, sizeof(unsigned) * s->ctas);
+    if (e == cudaSuccess) e = cudaMemset(s->cnt, 0, sizeof(unsigned) * s->ctas);
+    if (e == cudaSuccess) e = cudaDeviceSynchronize();
+    return e;
+}
+
+int qdb_paged_map(CUtensorMap *map, const void *pool, const QdbPagedKV &kv, int type, int rows) {
+    static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult qr;
+        const bool ok = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &qr) == cudaSuccess &&
+                        qr == cudaDriverEntryPointSuccess;
+        return ok ? (PFN_cuTensorMapEncodeTiled_v12000)p : nullptr;
+    }();
+    if (!fn) return -1;
+    const cuuint64_t dims[5] = {64, (cuuint64_t)1 << kv.page_shift, 2, (cuuint64_t)kv.kv_heads, (cuuint64_t)kv.n_pages};
+    const cuuint64_t strides[4] = {(cuuint64_t)kv.pos_stride * 2, 128, (cuuint64_t)kv.head_stride * 2,
+                                   (cuuint64_t)kv.page_stride * 2};
+    const cuuint32_t box[5] = {64, (cuuint32_t)rows, 2, 1, 1}, es[5] = {1, 1, 1, 1, 1};
+    return fn(map, type == QDB_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5,
+              const_cast<void *>(pool), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+               ? 0
+               : -1;
 }
 
 // ---------------------------------------------------------------- C entry points
@@ -295,6 +324,7 @@ static int launched(const char *fn, cudaError_t e) {
 // Workspace of the one-token attention.
 struct qdb_paged_workspace {
     int device;
+    QdbDecodeScratch s;
 };
 
 extern "C" qdb_paged_workspace *qdb_paged_workspace_create(int device) {
@@ -306,10 +336,28 @@ extern "C" qdb_paged_workspace *qdb_paged_workspace_create(int device) {
         qdb_set_error(m);
         return nullptr;
     }
-    return new qdb_paged_workspace{device};
+    qdb_paged_workspace *ws = new qdb_paged_workspace{device, {}};
+    int before = 0;
+    cudaGetDevice(&before);
+    cudaError_t e = cudaSetDevice(device);
+    if (e == cudaSuccess) e = qdb_decode_scratch_alloc(device, &ws->s);
+    cudaSetDevice(before);
+    if (e != cudaSuccess) {
+        char m[160];
+        snprintf(m, sizeof(m), "qdb_paged_workspace_create: %s", cudaGetErrorString(e));
+        qdb_set_error(m);
+        qdb_paged_workspace_free(ws);
+        return nullptr;
+    }
+    return ws;
 }
 
-extern "C" void qdb_paged_workspace_free(qdb_paged_workspace *ws) { delete ws; }
+extern "C" void qdb_paged_workspace_free(qdb_paged_workspace *ws) {
+    if (!ws) return;
+    cudaFree(ws->s.part);  // (cudaFree waits for the device's work)
+    cudaFree(ws->s.cnt);
+    delete ws;
+}
 
 extern "C" int qdb_paged_append(const qdb_paged_kv *kv, const qdb_paged_batch *batch, const void *qkv, int src_type,
                                 long long row_stride, int heads, const float *q_norm, const float *k_norm, float eps,
@@ -380,7 +428,10 @@ extern "C" int qdb_paged_decode(const qdb_paged_kv *kv, const qdb_paged_batch *b
     REFUSE(!ws, "%s: null workspace", fn);
     const int rc = check_attn(fn, kv, batch, q, q_stride, heads, scale, out, out_stride, &a);
     if (rc) return rc < 0 ? -1 : 0;
-    return launched(fn, qdb_launch_paged_decode(a, kv->type, (cudaStream_t)stream));
+    int dev = 0;
+    cudaGetDevice(&dev);
+    REFUSE(ws->device != dev, "%s: the workspace is of device %d, the current device is %d", fn, ws->device, dev);
+    return launched(fn, qdb_launch_paged_decode(a, kv->type, ws->s, (cudaStream_t)stream));
 }
 
 extern "C" int qdb_paged_prompt(const qdb_paged_kv *kv, const qdb_paged_batch *batch, const void *q,

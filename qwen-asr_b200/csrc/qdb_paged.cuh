@@ -7,6 +7,7 @@
 // s * pos_stride + d, so both [page][head][slot][128] and
 // [page][slot][head][128] pools are read in place.
 #pragma once
+#include <cuda.h>
 #include <cuda_bf16.h>
 
 #include "../../include/qwen_asr_b200.h"
@@ -90,6 +91,56 @@ __device__ __forceinline__ int paged_page(const QdbPagedKV &kv, const QdbPagedBa
     return check_or_record(p >= 0 && p < kv.n_pages, bt.err, QDB_CHECK_PAGE, b, p) ? p : -1;
 }
 
+// ---- barriers and tensor copies ----
+__device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void bar_init(uint32_t bar, unsigned n) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(n) : "memory");
+}
+__device__ __forceinline__ void bar_expect(uint32_t bar, unsigned bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool bar_try(uint32_t bar, unsigned parity) {
+    uint32_t ok;
+    asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+                 : "=r"(ok)
+                 : "r"(bar), "r"(parity)
+                 : "memory");
+    return ok != 0;
+}
+// Bounded wait; false = ran out (recorded).
+__device__ __forceinline__ bool bar_wait(uint32_t bar, unsigned parity, int *err) {
+    if (bar_try(bar, parity)) return true;
+    const long long t0 = clock64();
+    while (!bar_try(bar, parity))
+        if (clock64() - t0 > QDB_SPIN_LIMIT_CYCLES) {
+            set_error(err, QDB_ERR_BARRIER_TIMEOUT);
+            return false;
+        }
+    return true;
+}
+__device__ __forceinline__ void fence_bar_init() {
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+}
+// Generic-proxy shared-memory accesses ordered before later asynchronous ones.
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// The pools as 5-dimensional tensors (64 dims, slot, dim half, head, page):
+// one copy brings `rows` slots of a page as two [rows][64] halves, each with
+// rows of 128 bytes in the 128-byte swizzle.
+__device__ __forceinline__ void load_page(uint32_t dst, const CUtensorMap *map, int slot, int head, int page,
+                                          uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, "
+        "%6}], [%7];" ::"r"(dst),
+        "l"(map), "r"(0), "r"(slot), "r"(0), "r"(head), "r"(page), "r"(bar)
+        : "memory");
+}
+// Host: writes that map. rows: slots per copy (at most the page size). 0 = ok.
+int qdb_paged_map(CUtensorMap *map, const void *pool, const QdbPagedKV &kv, int type, int rows);
+
 // ---- host checks: refuses host pointers and pointers of another device than
 // the current one (null pointers are left to the caller). 0 = ok.
 struct QdbNamedPtr {
@@ -124,7 +175,15 @@ struct QdbPagedAttnArgs {
     uint16_t *out;
     long long out_stride;
 };
-cudaError_t qdb_launch_paged_decode(const QdbPagedAttnArgs &a, int type, cudaStream_t st);
+// Scratch of one call at a time: partial results [2 * ctas][16][130] f32 and
+// [ctas] counters, zero between calls.
+struct QdbDecodeScratch {
+    float *part;
+    unsigned *cnt;
+    int ctas;
+};
+cudaError_t qdb_decode_scratch_alloc(int device, QdbDecodeScratch *s);  // on the current device
+cudaError_t qdb_launch_paged_decode(const QdbPagedAttnArgs &a, int type, const QdbDecodeScratch &ws, cudaStream_t st);
 cudaError_t qdb_launch_paged_prompt(const QdbPagedAttnArgs &a, int type, cudaStream_t st);
 
 struct QdbSampleArgs {
