@@ -435,7 +435,8 @@ void qdb_paged_workspace_free(qdb_paged_workspace *ws);
  * [rows, heads * 128] in the cache's type, q_stride / out_stride elements
  * between rows (0 = contiguous, multiples of 8); scale 0 = 1/sqrt(128). Query
  * head h reads key head h / (heads / kv_heads); at most 16 query heads per key
- * head. A sequence of length 0 gives a row of zeros. */
+ * head. A sequence of length 0 gives a row of zeros. The page tables together
+ * may span up to n_seqs * table_stride * page_size * kv_heads = 2^35. */
 int qdb_paged_decode(const qdb_paged_kv *kv, const qdb_paged_batch *batch, const void *q, long long q_stride,
                      int heads, float scale, void *out, long long out_stride, qdb_paged_workspace *ws, void *stream);
 

@@ -192,7 +192,8 @@ cudaError_t qdb_launch_paged_prompt(const QdbPagedAttnArgs &a, int type, cudaStr
 
 cudaError_t qdb_decode_scratch_alloc(int device, QdbDecodeScratch *s) {
     cudaError_t e = cudaDeviceGetAttribute(&s->ctas, cudaDevAttrMultiProcessorCount, device);
-    if (e == cudaSuccess) e = cudaMalloc((void **)&s->part, sizeof(float) * 2 * s->ctas * 16 * 130);
+    if (e == cudaSuccess) e = cudaMalloc((void **)&s->part, sizeof(float) * 2 * s->ctas * 16 * QDB_HD);
+    if (e == cudaSuccess) e = cudaMalloc((void **)&s->ml, sizeof(float2) * 2 * s->ctas * 16);
     if (e == cudaSuccess) e = cudaMalloc((void **)&s->cnt, sizeof(unsigned) * s->ctas);
     if (e == cudaSuccess) e = cudaMemset(s->cnt, 0, sizeof(unsigned) * s->ctas);
     if (e == cudaSuccess) e = cudaDeviceSynchronize();
@@ -355,6 +356,7 @@ extern "C" qdb_paged_workspace *qdb_paged_workspace_create(int device) {
 extern "C" void qdb_paged_workspace_free(qdb_paged_workspace *ws) {
     if (!ws) return;
     cudaFree(ws->s.part);  // (cudaFree waits for the device's work)
+    cudaFree(ws->s.ml);
     cudaFree(ws->s.cnt);
     delete ws;
 }
@@ -430,6 +432,9 @@ extern "C" int qdb_paged_decode(const qdb_paged_kv *kv, const qdb_paged_batch *b
     if (rc) return rc < 0 ? -1 : 0;
     int dev = 0;
     cudaGetDevice(&dev);
+    REFUSE((double)batch->n_seqs * batch->table_stride * kv->page_size / 16 * kv->kv_heads >= 2147483648.0,
+           "%s: %d page tables of %d entries are too many positions for one call", fn, batch->n_seqs,
+           batch->table_stride);
     REFUSE(ws->device != dev, "%s: the workspace is of device %d, the current device is %d", fn, ws->device, dev);
     return launched(fn, qdb_launch_paged_decode(a, kv->type, ws->s, (cudaStream_t)stream));
 }

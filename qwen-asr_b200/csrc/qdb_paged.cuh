@@ -175,10 +175,11 @@ struct QdbPagedAttnArgs {
     uint16_t *out;
     long long out_stride;
 };
-// Scratch of one call at a time: partial results [2 * ctas][16][130] f32 and
-// [ctas] counters, zero between calls.
+// Scratch of one call at a time: partial results [2 * ctas][16][128] with their
+// (m, l), and [ctas] counters, zero between calls.
 struct QdbDecodeScratch {
     float *part;
+    float2 *ml;
     unsigned *cnt;
     int ctas;
 };

@@ -28,27 +28,38 @@ constexpr int DW = 8;             // warps per CTA
 constexpr int TILE = 16;          // keys per tile (a page holds whole tiles)
 constexpr int TILE_B = 4096;      // bytes of a tile's K (or V)
 constexpr int MAX_G = 16;         // query heads per key head
+#ifndef QDB_PD_MIN
+#define QDB_PD_MIN 8  // tiles of a CTA, on average, below which a pair is not cut further
+#endif
 constexpr float P_SHIFT = 8.0f;   // P is scaled by 2^8: f16 keeps weights down to 2^-32 of the largest
 
 // Ring stages per warp: what shared memory leaves beside one partial per warp.
 __host__ __device__ constexpr int ring_stages(int nt) { return nt == 1 ? 3 : 2; }
 
-// A pair whose parts are all there: sequence, key head, first CTA, CTAs.
-struct Whole {
-    bool some;
-    int b, g, c0, parts;
+// A pair with parts in this CTA: those of warps w0 (its last part, or where the
+// pair came from an earlier CTA its head part) to w1 (head parts), and the CTAs
+// c0 .. c1 that the pair lies in.
+struct Group {
+    int some, b, g, w0, w1, c0, c1;
 };
 
 template <int NT>
 struct DecodeSmem {
     static constexpr int NS = ring_stages(NT), H = 8 * NT;
     unsigned char ring[DW][NS][2][TILE_B];
-    float head_part[DW][H][QDB_HD];  // the part of a pair that began in an earlier warp
+    union {
+        float head_part[DW][H][QDB_HD];  // the part of a pair that began in an earlier warp
+        struct {  // until the warps have found their first tiles
+            int before[DW * 32];  // tiles of one key head ahead of each thread's share of the sequences
+            int len0[DW * 32];    // length of the share's first sequence
+        } find;
+    };
     float2 ml[DW][2][H];             // (m, l) of the head part and of the last part
     unsigned long long full[DW][NS];
-    long long scan[DW];
-    int start[DW][3];                // sequence, key head, tile of each warp's first tile
-    Whole todo;
+    int scan[DW];
+    int start[4];                    // warp 0's first tile: sequence, key head, tile; the sequence's length
+    Group grp[DW + 1];               // 0: came from an earlier CTA; 1 + w: begins in warp w and goes on
+    int todo[2];                     // groups whose last part arrived here (-1: none)
 };
 
 __device__ __forceinline__ void ldsm4(uint32_t *r, uint32_t a) {
@@ -89,23 +100,44 @@ struct Cursor {
     int b, g, tile, nt, len;
 };
 
-// One joined part: head h's (m, l) and this lane's 4 dims.
-struct Join {
-    float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-    __device__ __forceinline__ void add(float2 ml, float4 x) {
-        const float mn = fmaxf(m, ml.x);
-        const float f = m == mn ? 1.f : ex2(m - mn), w = ml.x == mn ? 1.f : ex2(ml.x - mn);
-        l = l * f + ml.y * w;
-        o[0] = o[0] * f + x.x * w;
-        o[1] = o[1] * f + x.y * w;
-        o[2] = o[2] * f + x.z * w;
-        o[3] = o[3] * f + x.w * w;
-        m = mn;
-    }
+// Joins parts 0 .. n-1 of one head: ml(i) = (m, l), row(i) = this lane's 4 dims.
+// The weights 2^(m_i - max) are computed one part per lane, then every lane
+// adds up its dims in the order of the parts.
+struct Joined {
+    float m, l, o[4];
 };
+template <typename ML, typename Row>
+__device__ __forceinline__ Joined join(int n, int lane, ML ml, Row row) {
+    Joined j;
+    j.m = -INFINITY;
+    for (int i = lane; i < n; i += 32) j.m = fmaxf(j.m, ml(i).x);
+    j.m = warp_max(j.m);
+    j.l = 0.f;
+    j.o[0] = j.o[1] = j.o[2] = j.o[3] = 0.f;
+    for (int i0 = 0; i0 < n; i0 += 32) {
+        float w = 0.f, l = 0.f;
+        if (i0 + lane < n) {
+            const float2 x = ml(i0 + lane);
+            w = x.x == j.m ? 1.f : exp2f(x.x - j.m);  // (also where both are -inf)
+            l = x.y * w;
+        }
+        j.l += warp_sum(l);
+        const int k = min(32, n - i0);
+#pragma unroll 8
+        for (int i = 0; i < k; i++) {
+            const float4 x = row(i0 + i);
+            const float f = __shfl_sync(0xffffffffu, w, i);
+            j.o[0] = fmaf(x.x, f, j.o[0]);
+            j.o[1] = fmaf(x.y, f, j.o[1]);
+            j.o[2] = fmaf(x.z, f, j.o[2]);
+            j.o[3] = fmaf(x.w, f, j.o[3]);
+        }
+    }
+    return j;
+}
 
 template <typename T>
-__device__ __forceinline__ void store_row4(uint16_t *dst, const Join &j) {
+__device__ __forceinline__ void store_row4(uint16_t *dst, const Joined &j) {
     const float inv = j.l > 0.f ? 1.0f / j.l : (isnan(j.l) ? j.l : 0.f);
     *reinterpret_cast<uint2 *>(dst) =
         make_uint2(T::pack(j.o[0] * inv, j.o[1] * inv), T::pack(j.o[2] * inv, j.o[3] * inv));
@@ -126,87 +158,91 @@ __global__ void __launch_bounds__(DW * 32, 1)
         for (int s = 0; s < NS; s++) bar_init(full0 + 8 * s, 1);
         fence_bar_init();
     }
+    if (t == 0) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&mk) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&mv) : "memory");
+    }
     pdl_enter();
     const int step = a.bt.step ? *a.bt.step : 0;
     auto length = [&](int b) { return paged_len(a.bt, b, a.kv.page_shift, step); };
 
-    // ---- the list: tiles before each thread's share of the sequences
+    // ---- the list: tiles ahead of each thread's share of the sequences (the
+    // host has checked that every count fits 31 bits)
     const int per = (n + DW * 32 - 1) / (DW * 32), b0 = min(n, t * per), b1 = min(n, b0 + per);
-    long long mine = 0;
+    int mine = 0;
     for (int b = b0; b < b1; b++) {
         const int len = length(b);
+        if (b == b0) sm.find.len0[t] = len;
         mine += (len + TILE - 1) / TILE;
+        if (len == 0 && b % gridDim.x == blockIdx.x)  // the row of an empty sequence is zero
+            for (int i = 0; i < a.heads * QDB_HD / 8; i++)
+                *reinterpret_cast<uint4 *>(a.out + (size_t)b * a.out_stride + i * 8) = make_uint4(0u, 0u, 0u, 0u);
     }
-    long long upto = mine;
+    int upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const long long y = __shfl_up_sync(0xffffffffu, upto, o);
+        const int y = __shfl_up_sync(0xffffffffu, upto, o);
         if (lane >= o) upto += y;
     }
     if (lane == 31) sm.scan[warp] = upto;
+    if (t <= DW) sm.grp[t].some = 0;
+    if (t < 2) sm.todo[t] = -1;
     __syncthreads();
-    long long total = 0, before = 0;
+    int total = 0, before = upto - mine;
+#pragma unroll
     for (int w = 0; w < DW; w++) {
-        if (w < warp) before += sm.scan[w];
-        total += sm.scan[w];
+        const int x = sm.scan[w];
+        if (w < warp) before += x;
+        total += x;
     }
-    before += upto - mine;
+    sm.find.before[t] = before;
     total *= Hkv;
-    // rows of empty sequences are zero
-    for (int b = blockIdx.x; b < n; b += gridDim.x)
-        if (length(b) == 0)
-            for (int i = t; i < a.heads * (QDB_HD / 8); i += DW * 32)
-                *reinterpret_cast<uint4 *>(a.out + (size_t)b * a.out_stride + i * 8) = make_uint4(0u, 0u, 0u, 0u);
     if (total == 0) return;
     // CTAs that take part: all of them where there are more pairs than CTAs;
-    // else a whole number per pair (equal lengths then need no join across
-    // CTAs beyond the pair's own), each with at least 32 tiles (512 keys) on
-    // average, below which a join costs more than the shorter range saves
-    const long long avg = total / ((long long)n * Hkv);
-    const long long np = (long long)n * Hkv;
+    // else a whole number per pair (equal lengths then need no join beyond the
+    // pair's own), each with at least QDB_PD_MIN tiles on average; never so many
+    // that a warp would have no tile (a range is empty only where one CTA does
+    // it all)
     int ctas = ws.ctas;
-    if (np <= ws.ctas) {
-        long long k = avg / 32;
-        if (k < 1) k = 1;
-        if (k > ws.ctas / np) k = ws.ctas / np;
-        ctas = (int)(np * k);
+    if ((long long)n * Hkv <= ctas) {
+        const int np = n * Hkv;
+        ctas = np * max(1, min(ctas / np, total / (np * QDB_PD_MIN)));
     }
-    // (a tile for every warp: a range is empty only where one CTA does it all)
-    if (ctas > total / DW) ctas = total >= DW ? (int)(total / DW) : 1;
+    ctas = min(ctas, max(total / DW, 1));
     if ((int)blockIdx.x >= ctas) return;
-    const long long nw = (long long)ctas * DW;
-    auto first_of = [&](long long w) { return total * w / nw; };  // first tile of global warp w's range
-    auto warp_of = [&](long long x) { return ((x + 1) * nw + total - 1) / total - 1; };  // its inverse
-    const long long gw0 = (long long)blockIdx.x * DW;
-    for (int w = 0; w < DW; w++) {
-        const long long x = first_of(gw0 + w);
-        if (x >= before * Hkv && x < (before + mine) * Hkv) {
-            long long at = before * Hkv;
-            for (int b = b0; b < b1; b++) {
-                const int nt = (length(b) + TILE - 1) / TILE;
-                if (x < at + (long long)nt * Hkv) {
-                    sm.start[w][0] = b;
-                    sm.start[w][1] = (int)((x - at) / nt);
-                    sm.start[w][2] = (int)((x - at) % nt);
-                    break;
-                }
-                at += (long long)nt * Hkv;
-            }
-        }
-    }
+    // warp w of the whole grid begins at tile first_of(w): share + 1 tiles for
+    // each of the first `more` warps, share for the rest
+    const int nw = ctas * DW, share = total / nw, more = total - share * nw;
+    auto first_of = [&](int w) { return share * w + min(w, more); };
+    auto cta_of = [&](int x) {  // the CTA whose range holds tile x
+        const int y = more * (share + 1);
+        return (x < y ? x / (share + 1) : more + (x - y) / share) / DW;
+    };
+    const int gw0 = blockIdx.x * DW, x0 = first_of(gw0 + warp), count = first_of(gw0 + warp + 1) - x0;
     __syncthreads();
 
-    const long long x0 = first_of(gw0 + warp), x1 = first_of(gw0 + warp + 1);
-    const int count = (int)(x1 - x0);
     // ---- copies: lane 0 issues tile i + NS when tile i has been used
-    Cursor pc, cc;
-    auto seek = [&](Cursor &c) {  // the warp's first tile
-        c.b = sm.start[warp][0];
-        c.g = sm.start[warp][1];
-        c.tile = sm.start[warp][2];
-        c.len = length(c.b);
-        c.nt = (c.len + TILE - 1) / TILE;
-    };
+    Cursor pc{}, cc{};
+    if (count > 0) {  // the warp's first tile: the last share that begins at or before it
+        int i = 0;
+#pragma unroll
+        for (int d = DW * 16; d; d >>= 1)
+            if (sm.find.before[i + d] * Hkv <= x0) i += d;
+        int rel = x0 - sm.find.before[i] * Hkv, b = min(n, i * per), len = sm.find.len0[i], nt = (len + TILE - 1) / TILE;
+        while (rel >= nt * Hkv) {
+            rel -= nt * Hkv;
+            len = length(++b);
+            nt = (len + TILE - 1) / TILE;
+        }
+        pc = Cursor{b, rel / nt, rel % nt, nt, len};
+        cc = pc;
+        if (t == 0) {
+            sm.start[0] = pc.b;
+            sm.start[1] = pc.g;
+            sm.start[2] = pc.tile;
+            sm.start[3] = pc.len;
+        }
+    }
     auto advance = [&](Cursor &c) {
         if (++c.tile < c.nt) return;
         c.tile = 0;
@@ -234,15 +270,23 @@ __global__ void __launch_bounds__(DW * 32, 1)
     };
     int issued = 0, next_page = 0;
     if (count > 0) {
-        seek(pc);
-        cc = pc;
-        if (lane == 0)
-            for (; issued < min(NS, count); issued++) {
-                issue(issued, pc, page_of(pc));
-                advance(pc);
-            }
-        if (lane == 0 && issued < count) next_page = page_of(pc);
+        // the first NS tiles' pages, and the one after them, are looked up side by side
+        int page = 0;
+        if (lane <= NS && lane < count) {
+            for (int i = 0; i < lane; i++) advance(pc);
+            page = page_of(pc);
+            if (lane < NS) issue(lane, pc, page);
+        }
+        issued = min(NS, count);
+        const int from = min(NS, count - 1);  // the cursor that goes on: tile NS
+        pc.b = __shfl_sync(0xffffffffu, pc.b, from);
+        pc.g = __shfl_sync(0xffffffffu, pc.g, from);
+        pc.tile = __shfl_sync(0xffffffffu, pc.tile, from);
+        pc.nt = __shfl_sync(0xffffffffu, pc.nt, from);
+        pc.len = __shfl_sync(0xffffffffu, pc.len, from);
+        next_page = __shfl_sync(0xffffffffu, page, from);
     }
+    __syncthreads();  // (`find` makes room for head_part)
 
     // ---- compute
     const float c = a.scale * 1.4426950408889634f;
@@ -252,7 +296,7 @@ __global__ void __launch_bounds__(DW * 32, 1)
     bool alive = true;
     int used = 0;
     bool has_head = false, has_last = false;  // partial results left in shared memory
-    long long pair_lo = x0 - (count > 0 ? cc.tile : 0);  // list position of the current pair's first tile
+    int pair_lo = x0 - (count > 0 ? cc.tile : 0);  // list position of the current pair's first tile
     const uint32_t krow = (lane & 7) + ((lane >> 3) & 1) * 8, kch = lane >> 4;
     const uint32_t vrow = (lane & 7) + (lane >> 4) * 8, vch = (lane >> 3) & 1;
     for (int i = 0; i < count && alive; i++) {
@@ -413,107 +457,74 @@ __global__ void __launch_bounds__(DW * 32, 1)
     // a wait that ran out: the copies in flight land before the CTA goes on
     if (!alive && lane == 0)
         for (int i = used; i < issued; i++) bar_wait(full0 + 8 * (i % NS), (i / NS) & 1, a.bt.err);
-    __syncthreads();
 
-    // ---- join. The pair list positions of this warp's first and last pair
-    // decide who joins: warp w the pair that begins in it and goes on behind
-    // it, warp 0 also the one that came from an earlier CTA.
-    const long long cta_lo = first_of(gw0), cta_hi = first_of(gw0 + DW);
-    for (int turn = 0; turn < 2; turn++) {
-        // turn 0: parts that began in an earlier CTA (warp 0's head part);
-        // turn 1: pairs that begin in this warp's range and go on behind it
-        Whole whole{false, 0, 0, 0, 0};
-        const bool act = turn == 0 ? (warp == 0 && has_head) : has_last;
-        int pb = 0, pg = 0, pnt = 0;
-        long long lo = 0;
-        if (act) {
-            if (turn == 0) {
-                pb = sm.start[0][0];
-                pg = sm.start[0][1];
-                lo = x0 - sm.start[0][2];
+    // ---- join: first the parts of this CTA, head by head over all warps
+    if (lane == 0 && ((warp == 0 && has_head) || has_last)) {
+        const int begin = first_of(gw0), end = first_of(gw0 + DW);
+        auto put = [&](Group &gr, int b, int g, int w0, int lo, int len) {
+            const int hi = lo + (len + TILE - 1) / TILE;
+            int w1 = w0;
+            while (w1 + 1 < DW && first_of(gw0 + w1 + 1) < hi) w1++;
+            gr = Group{1, b, g, w0, w1, lo < begin ? cta_of(lo) : (int)blockIdx.x, hi > end ? cta_of(hi - 1) : (int)blockIdx.x};
+        };
+        if (warp == 0 && has_head) put(sm.grp[0], sm.start[0], sm.start[1], 0, x0 - sm.start[2], sm.start[3]);
+        if (has_last) put(sm.grp[1 + warp], cc.b, cc.g, warp, x0 + count - 1 - cc.tile, cc.len);
+    }
+    __syncthreads();
+    auto out_row = [&](const Group &gr, int h) {
+        return a.out + (size_t)gr.b * a.out_stride + ((size_t)gr.g * G + h) * QDB_HD + lane * 4;
+    };
+    const unsigned groups = __ballot_sync(0xffffffffu, lane <= DW && sm.grp[lane <= DW ? lane : 0].some);
+    const bool split = __any_sync(0xffffffffu, (groups >> lane & 1) && sm.grp[lane].c0 != sm.grp[lane].c1);
+    int item = 0;
+    for (unsigned left = groups; left; left &= left - 1) {
+        const int k = __ffs(left) - 1;
+        for (int h = 0; h < G; h++, item++) {
+            if (item % DW != warp) continue;
+            const Group gr = sm.grp[k];
+            const Joined j = join(
+                gr.w1 - gr.w0 + 1, lane,
+                [&](int i) { return sm.ml[gr.w0 + i][i == 0 && k ? 1 : 0][h]; },
+                [&](int i) {
+                    const float *src = i == 0 && k ? reinterpret_cast<const float *>(&sm.ring[gr.w0][0][0][0])
+                                                   : &sm.head_part[gr.w0 + i][0][0];
+                    return *reinterpret_cast<const float4 *>(src + h * QDB_HD + lane * 4);
+                });
+            if (gr.c0 == gr.c1) {
+                store_row4<T>(out_row(gr, h), j);
             } else {
-                pb = cc.b;
-                pg = cc.g;
-                lo = x1 - 1 - cc.tile;
-            }
-            pnt = (length(pb) + TILE - 1) / TILE;
-            const long long hi = lo + pnt;
-            const long long last_w = warp_of(min(hi, cta_hi) - 1) - gw0;  // last warp of this CTA with a part
-            const bool inside = lo >= cta_lo && hi <= cta_hi;
-            const int c0 = (int)(warp_of(lo) / DW), c1 = (int)(warp_of(hi - 1) / DW);
-            for (int h = 0; h < G; h++) {
-                Join j;
-                const float *src = turn ? reinterpret_cast<const float *>(ring) : &sm.head_part[0][0][0];
-                j.add(sm.ml[warp][turn][h], *reinterpret_cast<const float4 *>(src + h * QDB_HD + lane * 4));
-                for (int w = warp + 1; w <= (int)last_w; w++) {
-                    if (first_of(gw0 + w) == first_of(gw0 + w + 1)) continue;  // an empty range
-                    j.add(sm.ml[w][0][h], *reinterpret_cast<const float4 *>(&sm.head_part[w][h][lane * 4]));
-                }
-                if (inside) {
-                    store_row4<T>(a.out + (size_t)pb * a.out_stride + ((size_t)pg * G + h) * QDB_HD + lane * 4, j);
-                } else {
-                    float *g = ws.part + ((size_t)(blockIdx.x * 2 + turn) * MAX_G + h) * 130;
-                    *reinterpret_cast<float2 *>(g + lane * 4) = make_float2(j.o[0], j.o[1]);
-                    *reinterpret_cast<float2 *>(g + lane * 4 + 2) = make_float2(j.o[2], j.o[3]);
-                    if (lane == 0) *reinterpret_cast<float2 *>(g + QDB_HD) = make_float2(j.m, j.l);
-                }
-            }
-            if (!inside) {
-                __threadfence();
-                __syncwarp();
-                unsigned seen = 0;
-                if (lane == 0) seen = atomicAdd(&ws.cnt[c0], 1u);
-                seen = __shfl_sync(0xffffffffu, seen, 0);
-                if (seen == (unsigned)(c1 - c0)) {  // the last of its parts
-                    __threadfence();
-                    whole = Whole{true, pb, pg, c0, c1 - c0 + 1};
-                }
+                const size_t at = (size_t)(blockIdx.x * 2 + (k ? 1 : 0)) * MAX_G + h;
+                *reinterpret_cast<float4 *>(ws.part + at * QDB_HD + lane * 4) = make_float4(j.o[0], j.o[1], j.o[2], j.o[3]);
+                if (lane == 0) ws.ml[at] = make_float2(j.m, j.l);
             }
         }
-        // at most one warp has a pair to finish in each turn: the whole CTA does it
-        if (t == 0) sm.todo.some = false;
-        __syncthreads();
-        if (whole.some && lane == 0) sm.todo = whole;
-        __syncthreads();
-        if (sm.todo.some) {
-            const Whole wd = sm.todo;
-            // warp: head warp % G and every pgc-th part, or heads warp, warp + 8, ...
-            const int pgc = G <= DW ? DW / G : 1;
-            float *sp = reinterpret_cast<float *>(&sm.ring[0][0][0][0] + 8192);  // free by now: [pgc][G][132]
-            for (int h = G <= DW ? warp % G : warp; h < G; h += DW) {
-                const int pg = G <= DW ? warp / G : 0;
-                Join j;
-                if (pg < pgc)
-#pragma unroll 4
-                    for (int i = pg; i < wd.parts; i += pgc) {
-                        const float *g = ws.part + ((size_t)((wd.c0 + i) * 2 + (i == 0 ? 1 : 0)) * MAX_G + h) * 130;
-                        const float2 x = __ldcg(reinterpret_cast<const float2 *>(g + lane * 4));
-                        const float2 y = __ldcg(reinterpret_cast<const float2 *>(g + lane * 4 + 2));
-                        j.add(__ldcg(reinterpret_cast<const float2 *>(g + QDB_HD)), make_float4(x.x, x.y, y.x, y.y));
-                    }
-                uint16_t *dst = a.out + (size_t)wd.b * a.out_stride + ((size_t)wd.g * G + h) * QDB_HD + lane * 4;
-                if (pgc == 1) {
-                    store_row4<T>(dst, j);
-                } else if (pg < pgc) {
-                    float *x = sp + (pg * G + h) * 132;
-                    *reinterpret_cast<float4 *>(x + lane * 4) = make_float4(j.o[0], j.o[1], j.o[2], j.o[3]);
-                    if (lane == 0) *reinterpret_cast<float2 *>(x + QDB_HD) = make_float2(j.m, j.l);
-                }
-            }
-            if (pgc > 1) {
-                __syncthreads();
-                if (warp < G) {
-                    Join j;
-                    for (int i = 0; i < pgc; i++) {
-                        const float *x = sp + (i * G + warp) * 132;
-                        j.add(*reinterpret_cast<const float2 *>(x + QDB_HD), *reinterpret_cast<const float4 *>(x + lane * 4));
-                    }
-                    store_row4<T>(a.out + (size_t)wd.b * a.out_stride + ((size_t)wd.g * G + warp) * QDB_HD + lane * 4, j);
-                }
-            }
-            if (t == 0) ws.cnt[wd.c0] = 0;
+    }
+    if (!split) return;
+    // ---- pairs over several CTAs (at most the first and the last of this one):
+    // the CTA whose part arrives last joins them
+    __threadfence();
+    __syncthreads();
+    if (t <= DW && sm.grp[t].some && sm.grp[t].c0 != sm.grp[t].c1) {
+        const Group gr = sm.grp[t];
+        if (atomicAdd(&ws.cnt[gr.c0], 1u) == (unsigned)(gr.c1 - gr.c0)) {
+            sm.todo[t ? 1 : 0] = t;
+            ws.cnt[gr.c0] = 0;  // nobody else comes
         }
-        __syncthreads();
+        __threadfence();
+    }
+    __syncthreads();
+    item = 0;
+    for (int k = 0; k < 2; k++) {
+        if (sm.todo[k] < 0) continue;
+        const Group gr = sm.grp[sm.todo[k]];
+        for (int h = 0; h < G; h++, item++) {
+            if (item % DW != warp) continue;
+            auto at = [&](int i) { return (size_t)((gr.c0 + i) * 2 + (i == 0 ? 1 : 0)) * MAX_G + h; };
+            const Joined j = join(
+                gr.c1 - gr.c0 + 1, lane, [&](int i) { return __ldcg(ws.ml + at(i)); },
+                [&](int i) { return __ldcg(reinterpret_cast<const float4 *>(ws.part + at(i) * QDB_HD + lane * 4)); });
+            store_row4<T>(out_row(gr, h), j);
+        }
     }
 }
 
