@@ -100,76 +100,6 @@ __global__ void append_kernel(const QdbAppendArgs a) {
     for (int i = 0; i < 4; i++) dst[lane + 32 * i] = T::one(e[i]);
 }
 
-// ---------------------------------------------------------------- attention
-// One warp per (row, query head), 32 keys at a time: lane j scores key j over
-// all 128 dims, then every lane sums 4 output dims over the 32 keys. Running
-// maximum and sum in f32.
-template <typename T>
-__global__ void attn_simple_kernel(const QdbPagedAttnArgs a) {
-    pdl_enter();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int row = blockIdx.x, head = blockIdx.y * (blockDim.x >> 5) + warp;
-    if (head >= a.heads) return;
-    const int b = row_sequence(a.bt, row);
-    if (b >= a.bt.n_seqs) return;
-    int first, last;
-    paged_rows(a.bt, b, first, last);
-    if (row < first || row >= last) return;
-    const int len = paged_len(a.bt, b, a.kv.page_shift, a.bt.step ? *a.bt.step : 0);
-    const int n = len - (last - 1 - row);  // keys this row sees
-    const int g = head / (a.heads / a.kv.kv_heads);
-    __shared__ __align__(16) float qs[8][QDB_HD];
-    const uint16_t *q = a.q + (size_t)row * a.q_stride + (size_t)head * QDB_HD;
-    for (int i = lane; i < QDB_HD; i += 32) qs[warp][i] = T::lo(q[i]) * a.scale;
-    __syncwarp();
-    float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int k0 = 0; k0 < n; k0 += 32) {
-        const int key = k0 + lane;
-        float s = -INFINITY;
-        long long at = -1;
-        if (key < n) {
-            const int page = paged_page(a.kv, a.bt, b, key >> a.kv.page_shift);
-            if (page >= 0) {
-                at = page * a.kv.page_stride + g * a.kv.head_stride +
-                     (key & ((1 << a.kv.page_shift) - 1)) * a.kv.pos_stride;
-                s = 0.f;
-                for (int d = 0; d < QDB_HD; d += 8) {
-                    const uint4 w = *reinterpret_cast<const uint4 *>(a.kv.k + at + d);
-                    const float *x = qs[warp] + d;
-                    s += T::lo(w.x) * x[0] + T::hi(w.x) * x[1] + T::lo(w.y) * x[2] + T::hi(w.y) * x[3] +
-                         T::lo(w.z) * x[4] + T::hi(w.z) * x[5] + T::lo(w.w) * x[6] + T::hi(w.w) * x[7];
-                }
-            }
-        }
-        const float mn = fmaxf(m, warp_max(s));
-        if (mn == -INFINITY) continue;
-        const float p = s == -INFINITY ? 0.f : expf(s - mn), f = m == -INFINITY ? 0.f : expf(m - mn);
-        m = mn;
-        l = l * f + warp_sum(p);
-#pragma unroll
-        for (int i = 0; i < 4; i++) o[i] *= f;
-        for (int j = 0; j < 32; j++) {
-            const long long aj = __shfl_sync(0xffffffffu, at, j);
-            const float pj = __shfl_sync(0xffffffffu, p, j);
-            if (aj < 0) continue;
-            const uint2 w = *reinterpret_cast<const uint2 *>(a.kv.v + aj + lane * 4);
-            o[0] += pj * T::lo(w.x);
-            o[1] += pj * T::hi(w.x);
-            o[2] += pj * T::lo(w.y);
-            o[3] += pj * T::hi(w.y);
-        }
-    }
-    const float inv = l > 0.f ? 1.0f / l : 0.f;
-    *reinterpret_cast<uint2 *>(a.out + (size_t)row * a.out_stride + (size_t)head * QDB_HD + lane * 4) =
-        make_uint2(T::pack(o[0] * inv, o[1] * inv), T::pack(o[2] * inv, o[3] * inv));
-}
-
-cudaError_t launch_simple(const QdbPagedAttnArgs &a, int type, cudaStream_t st) {
-    const dim3 grid(a.bt.rows, (a.heads + 7) / 8), block(256);
-    return type == QDB_TYPE_F16 ? pdl_launch(attn_simple_kernel<QdbHalf>, grid, block, 0, st, a)
-                                : pdl_launch(attn_simple_kernel<QdbBf16>, grid, block, 0, st, a);
-}
-
 }  // namespace
 
 cudaError_t qdb_launch_paged_append(const QdbAppendArgs &a, int src_type, int kv_type, cudaStream_t st) {
@@ -186,10 +116,6 @@ cudaError_t qdb_launch_paged_append(const QdbAppendArgs &a, int src_type, int kv
              : pdl_launch(append_kernel<QdbBf16, QdbBf16>, grid, block, 0, st, a);
 }
 
-cudaError_t qdb_launch_paged_prompt(const QdbPagedAttnArgs &a, int type, cudaStream_t st) {
-    return launch_simple(a, type, st);
-}
-
 cudaError_t qdb_decode_scratch_alloc(int device, QdbDecodeScratch *s) {
     cudaError_t e = cudaDeviceGetAttribute(&s->ctas, cudaDevAttrMultiProcessorCount, device);
     if (e == cudaSuccess) e = cudaMalloc((void **)&s->part, sizeof(float) * 2 * s->ctas * 16 * QDB_HD);
@@ -200,25 +126,38 @@ cudaError_t qdb_decode_scratch_alloc(int device, QdbDecodeScratch *s) {
     return e;
 }
 
-int qdb_paged_map(CUtensorMap *map, const void *pool, const QdbPagedKV &kv, int type, int rows) {
+static int encode_map(CUtensorMap *map, const void *p, int type, int rank, const cuuint64_t *dims,
+                      const cuuint64_t *strides, const cuuint32_t *box) {
     static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
-        void *p = nullptr;
+        void *f = nullptr;
         cudaDriverEntryPointQueryResult qr;
-        const bool ok = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &qr) == cudaSuccess &&
+        const bool ok = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &qr) == cudaSuccess &&
                         qr == cudaDriverEntryPointSuccess;
-        return ok ? (PFN_cuTensorMapEncodeTiled_v12000)p : nullptr;
+        return ok ? (PFN_cuTensorMapEncodeTiled_v12000)f : nullptr;
     }();
     if (!fn) return -1;
+    const cuuint32_t es[5] = {1, 1, 1, 1, 1};
+    return fn(map, type == QDB_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank,
+              const_cast<void *>(p), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+               ? 0
+               : -1;
+}
+
+int qdb_paged_map(CUtensorMap *map, const void *pool, const QdbPagedKV &kv, int type, int rows, int halves) {
     const cuuint64_t dims[5] = {64, (cuuint64_t)1 << kv.page_shift, 2, (cuuint64_t)kv.kv_heads, (cuuint64_t)kv.n_pages};
     const cuuint64_t strides[4] = {(cuuint64_t)kv.pos_stride * 2, 128, (cuuint64_t)kv.head_stride * 2,
                                    (cuuint64_t)kv.page_stride * 2};
-    const cuuint32_t box[5] = {64, (cuuint32_t)rows, 2, 1, 1}, es[5] = {1, 1, 1, 1, 1};
-    return fn(map, type == QDB_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5,
-              const_cast<void *>(pool), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
-               ? 0
-               : -1;
+    const cuuint32_t box[5] = {64, (cuuint32_t)rows, (cuuint32_t)halves, 1, 1};
+    return encode_map(map, pool, type, 5, dims, strides, box);
+}
+
+int qdb_encode_map4(CUtensorMap *map, const void *q, int type, uint64_t heads, uint64_t rows, uint64_t row_stride,
+                    uint32_t box_heads, uint32_t box_rows) {
+    const cuuint64_t dims[4] = {64, 2, heads, rows};
+    const cuuint64_t strides[3] = {128, 256, row_stride * 2};
+    const cuuint32_t box[4] = {64, 1, box_heads, box_rows};
+    return encode_map(map, q, type, 4, dims, strides, box);
 }
 
 // ---------------------------------------------------------------- C entry points

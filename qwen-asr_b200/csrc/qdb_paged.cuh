@@ -47,6 +47,20 @@ struct QdbHalf {
         return (uint32_t)one(a) | ((uint32_t)one(b) << 16);
     }
     static __device__ __forceinline__ uint16_t one(float f) { return isnan(f) ? (uint16_t)0x7fffu : f32_to_kv(f); }
+    // without saturation: infinities stay
+    static __device__ __forceinline__ uint16_t plain1(float f) { return __half_as_ushort(__float2half_rn(f)); }
+    static __device__ __forceinline__ uint32_t plain(float a, float b) {
+        const __half2 r = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&r);
+    }
+    static __device__ __forceinline__ bool any_nonfinite(uint32_t w) {
+        return (w & 0x7c00u) == 0x7c00u || (w & 0x7c000000u) == 0x7c000000u;
+    }
+    static __device__ __forceinline__ uint32_t clear_nonfinite(uint32_t w) {
+        if ((w & 0x7c00u) == 0x7c00u) w &= 0xffff0000u;
+        if ((w & 0x7c000000u) == 0x7c000000u) w &= 0xffffu;
+        return w;
+    }
 };
 struct QdbBf16 {
     static constexpr int code = QDB_TYPE_BF16;
@@ -57,6 +71,16 @@ struct QdbBf16 {
         return *reinterpret_cast<const uint32_t *>(&r);
     }
     static __device__ __forceinline__ uint16_t one(float f) { return f32_to_bf16_rn(f); }
+    static __device__ __forceinline__ uint16_t plain1(float f) { return one(f); }
+    static __device__ __forceinline__ uint32_t plain(float a, float b) { return pack(a, b); }
+    static __device__ __forceinline__ bool any_nonfinite(uint32_t w) {
+        return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
+    }
+    static __device__ __forceinline__ uint32_t clear_nonfinite(uint32_t w) {
+        if ((w & 0x7f80u) == 0x7f80u) w &= 0xffff0000u;
+        if ((w & 0x7f800000u) == 0x7f800000u) w &= 0xffffu;
+        return w;
+    }
 };
 
 // Length of sequence b: never negative, never behind its page table.
@@ -138,8 +162,21 @@ __device__ __forceinline__ void load_page(uint32_t dst, const CUtensorMap *map, 
         "l"(map), "r"(0), "r"(slot), "r"(0), "r"(head), "r"(page), "r"(bar)
         : "memory");
 }
-// Host: writes that map. rows: slots per copy (at most the page size). 0 = ok.
-int qdb_paged_map(CUtensorMap *map, const void *pool, const QdbPagedKV &kv, int type, int rows);
+// One half only, from a map of one half per copy.
+__device__ __forceinline__ void load_half_page(uint32_t dst, const CUtensorMap *map, int slot, int half, int head,
+                                               int page, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, "
+        "%6}], [%7];" ::"r"(dst),
+        "l"(map), "r"(0), "r"(slot), "r"(half), "r"(head), "r"(page), "r"(bar)
+        : "memory");
+}
+// Host: writes that map. rows: slots per copy (at most the page size), halves: 1 or 2 per copy. 0 = ok.
+int qdb_paged_map(CUtensorMap *map, const void *pool, const QdbPagedKV &kv, int type, int rows, int halves);
+// Rows [rows][heads][128] of queries as (64 dims, dim half, head, row): a copy
+// brings one half of box_heads heads of box_rows rows.
+int qdb_encode_map4(CUtensorMap *map, const void *q, int type, uint64_t heads, uint64_t rows, uint64_t row_stride,
+                    uint32_t box_heads, uint32_t box_rows);
 
 // ---- host checks: refuses host pointers and pointers of another device than
 // the current one (null pointers are left to the caller). 0 = ok.

@@ -140,7 +140,7 @@ template <typename T>
 __device__ __forceinline__ void store_row4(uint16_t *dst, const Joined &j) {
     const float inv = j.l > 0.f ? 1.0f / j.l : (isnan(j.l) ? j.l : 0.f);
     *reinterpret_cast<uint2 *>(dst) =
-        make_uint2(T::pack(j.o[0] * inv, j.o[1] * inv), T::pack(j.o[2] * inv, j.o[3] * inv));
+        make_uint2(T::plain(j.o[0] * inv, j.o[1] * inv), T::plain(j.o[2] * inv, j.o[3] * inv));
 }
 
 template <typename T, int NT>
@@ -389,8 +389,8 @@ __global__ void __launch_bounds__(DW * 32, 1)
             v[3] = ex2(v[3] - a1);
             l[j][0] += v[0] + v[2];
             l[j][1] += v[1] + v[3];
-            p[j][0] = transpose8(T::pack(v[0], v[1]));
-            p[j][1] = transpose8(T::pack(v[2], v[3]));
+            p[j][0] = transpose8(T::plain(v[0], v[1]));
+            p[j][1] = transpose8(T::plain(v[2], v[3]));
         }
 #pragma unroll
         for (int mt = 0; mt < 8; mt++) {
@@ -427,8 +427,8 @@ __global__ void __launch_bounds__(DW * 32, 1)
                         const float inv = l[j][e] > 0.f ? 1.0f / l[j][e] : (isnan(l[j][e]) ? l[j][e] : 0.f);
 #pragma unroll
                         for (int mt = 0; mt < 8; mt++) {
-                            dst[h * QDB_HD + mt * 16 + qr] = T::one(o[mt][j][e] * inv);
-                            dst[h * QDB_HD + mt * 16 + 8 + qr] = T::one(o[mt][j][e + 2] * inv);
+                            dst[h * QDB_HD + mt * 16 + qr] = T::plain1(o[mt][j][e] * inv);
+                            dst[h * QDB_HD + mt * 16 + 8 + qr] = T::plain1(o[mt][j][e + 2] * inv);
                         }
                     }
             } else {
@@ -541,7 +541,7 @@ cudaError_t launch(const CUtensorMap &mk, const CUtensorMap &mv, const QdbPagedA
 
 cudaError_t qdb_launch_paged_decode(const QdbPagedAttnArgs &a, int type, const QdbDecodeScratch &ws, cudaStream_t st) {
     CUtensorMap mk, mv;
-    if (qdb_paged_map(&mk, a.kv.k, a.kv, type, TILE) || qdb_paged_map(&mv, a.kv.v, a.kv, type, TILE))
+    if (qdb_paged_map(&mk, a.kv.k, a.kv, type, TILE, 2) || qdb_paged_map(&mv, a.kv.v, a.kv, type, TILE, 2))
         return cudaErrorInvalidValue;
     const bool narrow = a.heads / a.kv.kv_heads <= 8;
     if (type == QDB_TYPE_F16)

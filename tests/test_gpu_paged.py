@@ -314,6 +314,30 @@ def test_prompt_rising_scores(pkg):
         check_attention(pool, q, run_prompt(pkg, pool, q, [n], scale=1 / 64), [n], scale=1 / 64)
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("key,q_len", [(100, 300), (0, 300), (299, 300), (5, 40), (270, 40), (128, 172)])
+def test_prompt_non_finite_values_reach_only_rows_that_see_them(pkg, dtype, key, q_len):
+    n = 300
+    pool = Pool(pkg, [n], 2, 32, dtype, seed=6)
+    q = queries(q_len, 4, dtype)
+    clean = run_prompt(pkg, pool, q, [q_len])
+    pg, sl = pool.where(0, n)
+    pool.v[pg[key], 1, sl[key], 3] = float("inf")
+    pool.v[pg[key], 1, sl[key], 9] = float("nan")
+    pool.v[pg[key], 1, sl[key], 127] = -float("inf")
+    out = run_prompt(pkg, pool, q, [q_len])
+    sees = torch.arange(n - q_len, n, device="cuda") >= key
+    assert torch.equal(out[~sees], clean[~sees])
+    assert torch.equal(out[:, :2], clean[:, :2])
+    bad = out[sees][:, 2:]
+    # inf times a weight: inf, or NaN where the weight is below the type's smallest
+    assert ((bad[..., 3] == float("inf")) | torch.isnan(bad[..., 3])).all()
+    assert ((bad[..., 127] == -float("inf")) | torch.isnan(bad[..., 127])).all()
+    assert torch.isnan(bad[..., 9]).all()
+    rest = [d for d in range(D) if d not in (3, 9, 127)]
+    assert torch.equal(bad[..., rest], clean[sees][:, 2:][..., rest])
+
+
 def test_prompt_equals_decode(pkg, ws):
     """The last row of a prompt is the decode row of the same cache."""
     pool = Pool(pkg, [500, 31, 1], 2, 16, "f16", seed=2)
