@@ -24,8 +24,10 @@
 //      the top_k or the top_p ends at the latest
 //   3. the tokens down to that bin, if at most 2048, go to the first CTA, which
 //      sorts them, cuts exactly, sorts the rest by index and draws
-// More tokens than that (a flat distribution) are cut by a radix selection on
-// the integers, digit by digit over the cluster, and drawn where they are. Both
+// Where more tokens than that may stay (a flat distribution), only the bins
+// that hold the end of the top_k, then of the top_p, go to the first CTA, which
+// finds the last token that stays; every CTA then draws from its own tokens.
+// Bins of more than 2048 (many equal logits) are cut by a radix selection. All
 // ways take the same integer weights, so they give the same token.
 #include <cooperative_groups.h>
 #include <math.h>
@@ -72,8 +74,13 @@ __device__ __forceinline__ X warp_scan(X v, int lane) {  // inclusive
 
 struct Pick {     // of one digit of the radix selection
     int digit;
-    unsigned above_n, ties;
+    unsigned ties;
     u64 above;    // count or weight above the digit
+};
+
+enum Way { ALL_LISTED, K_BIN, P_BINS, RADIX };
+struct Plan {     // what the CTAs do next: bins lo .. hi go to the list
+    int way, lo, hi;
 };
 
 struct SampleSmem {
@@ -82,23 +89,25 @@ struct SampleSmem {
             unsigned n[BINS];
             float w[BINS];
         } hist;
-        u64 list[LIST];
+        u64 val[LIST];
     };
     union {
-        u64 val[LIST];
+        u64 list[LIST];
         struct {
             u64 w[256], lead_w[256];
             unsigned n[256], lead_n[256];
         } dig;
     };
+    double exp2_64[64];  // 2^(45 + i / 64)
     u64 scan[SW + 1];
     float scan_f[SW + 1];
     u64 best[SC], total[SC];
     uint32_t low[SC];
-    unsigned ties[SC];
-    u64 weight;      // first CTA: sum of all weights
+    u64 weight;      // first CTA: a sum of weights
     unsigned count;  // first CTA: tokens in the list
-    int limit;       // last bin that goes to the list, -1: too many
+    u64 cut;         // the last token that stays
+    int lo, hi;      // first CTA
+    Plan plan;
     Pick pick;
 };
 
@@ -134,7 +143,7 @@ __device__ void sort_down(u64 *x, int n2, int t) {
 }
 
 template <int TYPE>
-__global__ void __launch_bounds__(ST) sample_kernel(const QdbSampleArgs a, int slice) {
+__global__ void __launch_bounds__(ST, 2) sample_kernel(const QdbSampleArgs a, int slice) {
     extern __shared__ __align__(16) unsigned char smem_raw[];
     SampleSmem &sm = *reinterpret_cast<SampleSmem *>(smem_raw);
     uint32_t *keys = reinterpret_cast<uint32_t *>(smem_raw + sizeof(SampleSmem));
@@ -145,6 +154,7 @@ __global__ void __launch_bounds__(ST) sample_kernel(const QdbSampleArgs a, int s
     SampleSmem *lead = cl.map_shared_rank(&sm, 0);
     for (int i = t; i < BINS; i += ST) sm.hist.n[i] = 0, sm.hist.w[i] = 0.f;
     if (t == 0) sm.weight = 0, sm.count = 0;
+    if (t < 64) sm.exp2_64[t] = exp2(45.0 + t / 64.0);
     cl.barrier_arrive();  // (waited for before the first access to another CTA's memory)
     pdl_enter();
     const size_t out_at = (a.step ? (size_t)*a.step * a.rows : 0) + row;
@@ -210,34 +220,81 @@ __global__ void __launch_bounds__(ST) sample_kernel(const QdbSampleArgs a, int s
     }
     const uint32_t kmax = (uint32_t)(best >> 32);
     const float fmax = key_logit(kmax);
-    const double lmax = (double)fmax, dT = (double)T, floor_w = (double)min_p;
+    const double lmax = (double)fmax, floor_w = (double)min_p * S_ONE;
     const bool k_on = top_k > 0 && top_k < V, p_on = top_p < 1.f, first = !(u > 0.f);
-    auto real_weight = [&](uint32_t k) { return k == kmax ? 1.0 : exp(((double)key_logit(k) - lmax) / dT); };
-    auto weight = [&](uint32_t k) -> u64 {  // in units of 2^-45
-        return k ? __double2ull_rn(real_weight(k) * S_ONE) : 0;
+    // 2^45 exp((l - max) / T) by 2^(i / 64) from the table times a polynomial of
+    // degree 4 in the rest (below 0.0055: the next term is 2^-44 of the weight)
+    const double c64 = 64.0 * 1.4426950408889634074 / (double)T;
+    auto real_weight = [&](uint32_t k) -> double {
+        if (k == kmax) return S_ONE;
+        const double d = (double)key_logit(k) - lmax, magic = 6755399441055744.0;  // 1.5 * 2^52
+        const double y = fma(d, c64, magic);
+        const int i = __double2loint(y);
+        const double x = fma(d, c64, magic - y) * (0.69314718055994530942 / 64.0);
+        double e = fma(x, 1.0 / 24, 1.0 / 6);
+        e = fma(x, e, 0.5);
+        e = fma(x, e, 1.0);
+        e = fma(x, e, 1.0) * sm.exp2_64[i & 63];
+        return __hiloint2double(__double2hiint(e) + ((i >> 6) << 20), __double2loint(e));
     };
+    auto whole_weight = [&](double w) -> u64 {  // rounded to an integer (below 2^51)
+        return (u64)__double_as_longlong(w + 4503599627370496.0) & ((1ull << 52) - 1);
+    };
+    auto weight = [&](uint32_t k) { return whole_weight(real_weight(k)); };
     const float reach = S_REACH * T;  // logits further below the maximum weigh nothing
     auto weightless = [&](uint32_t k) { return !k || (k != kmax && !(fmax - key_logit(k) <= reach)); };
+    auto token = [&](int i) { return (u64)keys[i] << 32 | (0xffffffffu - (uint32_t)(base + i)); };
+    auto warp_total = [&](u64 v) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        return v;
+    };
+    // Tokens that `take` wants to the first CTA's list (in any order); a
+    // barrier of the cluster has to follow.
+    auto gather = [&](auto take) {
+        for (int i0 = warp * 32; i0 < n; i0 += ST) {
+            const bool yes = i0 + lane < n && take(i0 + lane);
+            const unsigned m = __ballot_sync(0xffffffffu, yes);
+            if (!m) continue;
+            unsigned at = 0;
+            if (lane == 0) at = atomicAdd(&lead->count, __popc(m));
+            at = __shfl_sync(0xffffffffu, at, 0) + __popc(m & ((1u << lane) - 1));
+            if (yes && at < LIST) lead->list[at] = token(i0 + lane);
+        }
+    };
+    // First CTA: sorts the list; returns its length.
+    auto sort_list = [&](int *n2) {
+        const int m = min((int)sm.count, LIST);
+        *n2 = 32;
+        while (*n2 < m) *n2 <<= 1;
+        for (int i = m + t; i < *n2; i += ST) sm.list[i] = 0;
+        sort_down(sm.list, *n2, t);
+        return m;
+    };
+    constexpr int PT = BINS / ST;  // bins, or list entries, of a thread
+    u64 cut = 0;                   // tokens from here up stay
+    int way = RADIX;
 
     // ---- 2. histogram: how far down the kept tokens can go
+    const float span = fminf(reach, fmax - key_logit(low)), s = span > 0.f ? (float)BINS / span : 0.f;
+    auto bin_of = [&](uint32_t k) { return k == kmax ? 0 : min(BINS - 1, (int)((fmax - key_logit(k)) * s)); };
     if ((k_on || p_on) && !first) {
-        const float span = fminf(reach, fmax - key_logit(low)), s = span > 0.f ? (float)BINS / span : 0.f;
-        auto bin_of = [&](uint32_t k) { return k == kmax ? 0 : min(BINS - 1, (int)((fmax - key_logit(k)) * s)); };
+        const bool need_w = p_on && (!k_on || top_k > LIST);
         u64 sum = 0;
         const float c = -1.4426950408889634f / T;
+#pragma unroll 4
         for (int i = t; i < n; i += ST) {
             const uint32_t k = keys[i];
             if (weightless(k)) continue;
             const int b = bin_of(k);
             atomicAdd(&sm.hist.n[b], 1u);
-            if (!k_on) {
+            if (need_w) {
                 atomicAdd(&sm.hist.w[b], k == kmax ? 1.f : exp2f((fmax - key_logit(k)) * c));
-                sum += weight(k);
+                if (!k_on) sum += weight(k);
             }
         }
-        if (!k_on) {
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (p_on && !k_on) {
+            sum = warp_total(sum);
             if (lane == 0) atomicAdd(&lead->weight, sum);
         }
         __syncthreads();
@@ -245,62 +302,163 @@ __global__ void __launch_bounds__(ST) sample_kernel(const QdbSampleArgs a, int s
             for (int i = t; i < BINS; i += ST)
                 if (sm.hist.n[i]) {
                     atomicAdd(&lead->hist.n[i], sm.hist.n[i]);
-                    if (!k_on) atomicAdd(&lead->hist.w[i], sm.hist.w[i]);
+                    if (need_w) atomicAdd(&lead->hist.w[i], sm.hist.w[i]);
                 }
         cl.sync();
+        unsigned cn = 0, all_n;  // first CTA: tokens and (in f32) weight ahead of this thread's bins
+        float cw = 0.f, all_w;
+        // First CTA: bins lo .. hi that hold the end of the top_p for a given
+        // total weight. The f32 sums are taken to be off by up to 2^-11 (more only
+        // where bins hold thousands of tokens: what was found is checked).
+        auto p_bins = [&](u64 whole) {
+            const float goal = (float)((double)top_p * (double)whole / S_ONE);
+            float w = cw;
+            int lo = BINS - 1, hi = BINS - 1;
+#pragma unroll
+            for (int e = PT - 1; e >= 0; e--) {
+                float x = w;
+                for (int f = 0; f <= e; f++) x += sm.hist.w[t * PT + f];
+                if (x * (1.f + 1.f / 2048) >= goal) lo = t * PT + e;
+                if (x * (1.f - 1.f / 2048) >= goal) hi = t * PT + e;
+            }
+            if (t == 0) sm.lo = sm.hi = BINS - 1;
+            __syncthreads();
+            atomicMin(&sm.lo, lo);
+            atomicMin(&sm.hi, hi);
+            __syncthreads();
+        };
+        auto tell = [&](int way, int lo, int hi) {  // first CTA
+            if (t < C) cl.map_shared_rank(&sm, t)->plan = Plan{way, lo, hi};
+        };
         if (rank == 0) {
-            constexpr int PT = BINS / ST;
-            unsigned cn = 0, all_n;
-            float cw = 0.f, all_w;
 #pragma unroll
             for (int e = 0; e < PT; e++) cn += sm.hist.n[t * PT + e], cw += sm.hist.w[t * PT + e];
-            if (t == 0) sm.limit = BINS - 1;
             cn = block_scan<unsigned>(cn, reinterpret_cast<unsigned *>(sm.scan), lane, warp, &all_n);
             cw = block_scan<float>(cw, sm.scan_f, lane, warp, &all_w);
-            // (the f32 sums of up to 2048 bins of up to 2048 tokens are off by
-            // less than 2^-11; bins with more tokens end in the other way anyhow)
-            const float goal = (float)((double)top_p * (double)sm.weight / S_ONE) * (1.f + 1.f / 2048);
-            int lim = BINS;
+            if (k_on) {  // the bin in which the count is reached
+                int lim = BINS - 1;
+                unsigned x = cn;
 #pragma unroll
-            for (int e = 0; e < PT; e++) {
-                cn += sm.hist.n[t * PT + e];
-                cw += sm.hist.w[t * PT + e];
-                if (lim == BINS && (k_on ? cn >= (unsigned)top_k : cw >= goal)) lim = t * PT + e;
+                for (int e = 0; e < PT; e++) {
+                    x += sm.hist.n[t * PT + e];
+                    if (lim == BINS - 1 && x >= (unsigned)top_k) lim = t * PT + e;
+                }
+                if (t == 0) sm.hi = BINS - 1;
+                __syncthreads();
+                atomicMin(&sm.hi, lim);
+                __syncthreads();
+            } else {
+                p_bins(sm.weight);
             }
-            atomicMin(&sm.limit, lim);
+            // tokens down to hi, and in lo .. hi
+            const int hi = sm.hi, lo = k_on ? hi : sm.lo;
+            auto upto = [&](int bin, unsigned *dst) {
+                if (bin / PT != t) return;
+                unsigned x = cn;
+                for (int b = t * PT; b <= bin; b++) x += sm.hist.n[b];
+                *dst = x;
+            };
+            unsigned *to = reinterpret_cast<unsigned *>(sm.scan);
             __syncthreads();
-            const int limit = sm.limit;
-            if (limit / PT == t) {  // the tokens down to it
-                for (int e = PT - 1; t * PT + e > limit; e--) cn -= sm.hist.n[t * PT + e];
-                sm.count = cn;
-            }
+            if (t == 0) to[0] = 0;
             __syncthreads();
-            if (t < C) cl.map_shared_rank(&sm, t)->limit = sm.count > LIST ? -1 : limit;
+            upto(hi, to + 1);
+            if (lo > 0) upto(lo - 1, to);
             __syncthreads();
-            if (t == 0) sm.count = 0;
+            const unsigned ahead = to[0], down = to[1];
+            tell(down <= LIST ? ALL_LISTED : down - ahead > LIST ? RADIX : k_on ? K_BIN : P_BINS, lo, hi);
+            if (t == 0) sm.pick.above = ahead;
         }
         cl.sync();
-        const int limit = sm.limit;
-        if (limit >= 0) {
-            // ---- 3. those tokens to the first CTA
-            for (int i0 = warp * 32; i0 < n; i0 += ST) {
-                const uint32_t k = i0 + lane < n ? keys[i0 + lane] : 0u;
-                const bool take = !weightless(k) && bin_of(k) <= limit;
-                const unsigned m = __ballot_sync(0xffffffffu, take);
-                if (!m) continue;
-                unsigned at = 0;
-                if (lane == 0) at = atomicAdd(&lead->count, __popc(m));
-                at = __shfl_sync(0xffffffffu, at, 0) + __popc(m & ((1u << lane) - 1));
-                if (take && at < LIST) lead->list[at] = (u64)k << 32 | (0xffffffffu - (uint32_t)(base + i0 + lane));
+        way = sm.plan.way;
+        if (way == K_BIN) {  // the end of the top_k
+            const int bin = sm.plan.hi;
+            gather([&](int i) { return !weightless(keys[i]) && bin_of(keys[i]) == bin; });
+            cl.sync();
+            if (rank == 0) {
+                int n2;
+                const int m = sort_list(&n2);
+                const u64 last = sm.list[min(m, top_k - (int)sm.pick.above) - 1];
+                if (t < C) cl.map_shared_rank(&sm, t)->cut = last;
+                __syncthreads();
+                if (t == 0) sm.count = 0;
             }
             cl.sync();
+            cut = sm.cut;
+            if (top_k <= LIST) {
+                way = ALL_LISTED;
+            } else if (p_on) {  // the weight of the top_k, then the bins of the top_p
+                u64 w = 0;
+                for (int i = t; i < n; i += ST)
+                    if (!weightless(keys[i]) && token(i) >= cut) w += weight(keys[i]);
+                w = warp_total(w);
+                if (lane == 0) atomicAdd(&lead->weight, w);
+                cl.sync();
+                if (rank == 0) {
+                    p_bins(sm.weight);
+                    tell(P_BINS, sm.lo, sm.hi);
+                }
+                cl.sync();
+                way = P_BINS;
+            }
+        }
+        if (way == P_BINS) {  // the end of the top_p
+            const int lo = sm.plan.lo, hi = sm.plan.hi;
+            u64 w = 0;
+#pragma unroll 2
+            for (int i = t; i < n; i += ST) {
+                const uint32_t k = keys[i];
+                if (!weightless(k) && bin_of(k) < lo && token(i) >= cut) w += weight(k);
+            }
+            w = warp_total(w);
+            if (t == 0 && rank == 0) sm.total[0] = 0;
+            cl.sync();
+            if (lane == 0) atomicAdd(&lead->total[0], w);
+            gather([&](int i) {
+                if (weightless(keys[i]) || token(i) < cut) return false;
+                const int b = bin_of(keys[i]);
+                return b >= lo && b <= hi;
+            });
+            cl.sync();
+            if (rank == 0) {
+                int n2;
+                const bool fits = sm.count <= LIST;
+                const int m = sort_list(&n2);
+                u64 x[PT], mine = 0, all;
+#pragma unroll
+                for (int e = 0; e < PT; e++) {
+                    const int i = t * PT + e;
+                    x[e] = i < m ? weight((uint32_t)(sm.list[i] >> 32)) : 0;
+                    mine += x[e];
+                }
+                const u64 goal = (u64)ceil((double)top_p * (double)sm.weight), ahead = sm.total[0];
+                u64 before = ahead + block_scan<u64>(mine, sm.scan, lane, warp, &all);
+                const bool good = fits && m > 0 && ahead < goal && ahead + all >= goal;
+#pragma unroll
+                for (int e = 0; e < PT; e++) {
+                    if (x[e] && before < goal && before + x[e] >= goal && good) sm.cut = sm.list[t * PT + e];
+                    before += x[e];
+                }
+                __syncthreads();
+                const u64 last = sm.cut;
+                __syncthreads();
+                if (t < C) {
+                    cl.map_shared_rank(&sm, t)->cut = last;
+                    cl.map_shared_rank(&sm, t)->plan = Plan{good ? P_BINS : RADIX, 0, 0};
+                }
+            }
+            cl.sync();
+            way = sm.plan.way;
+            if (way == P_BINS) cut = sm.cut;
+        }
+        if (way == ALL_LISTED) {
+            // ---- 3. the tokens that may stay to the first CTA
+            const int hi = sm.plan.hi;
+            gather([&](int i) { return !weightless(keys[i]) && (cut ? token(i) >= cut : bin_of(keys[i]) <= hi); });
+            cl.sync();
             if (rank) return;
-            const int m = min((int)sm.count, LIST);
-            int n2 = 32;
-            while (n2 < m) n2 <<= 1;
-            for (int i = m + t; i < n2; i += ST) sm.list[i] = 0;
-            sort_down(sm.list, n2, t);
-            constexpr int PT = LIST / ST;
+            int n2;
+            const int m = sort_list(&n2);
             // (logit descending, index ascending): thread t has entries t * PT ..
             u64 w[PT], mine = 0, total;
 #pragma unroll
@@ -346,130 +504,121 @@ __global__ void __launch_bounds__(ST) sample_kernel(const QdbSampleArgs a, int s
         }
     }
 
-    // ---- many tokens: (cut, ties): keys above cut stay, and the first `ties`
-    // (by index) equal to it
-    uint32_t cut = 0;
-    unsigned ties = 0xffffffffu;
-    if ((k_on || p_on)) {
-        if (rank == 0)
-            for (int i = t; i < 256; i += ST) sm.dig.lead_n[i] = 0, sm.dig.lead_w[i] = 0;
-        cl.sync();
-    }
-    // Most significant digit first: the digit in which the running count (or
-    // weight) from the top reaches the target. Elements: keys >= lim.
-    auto select = [&](bool by_weight, u64 target, uint32_t lim, unsigned lim_ties) {
-        uint32_t prefix = 0;
-        u64 above = 0;
-        unsigned above_n = 0, n_tie = 0;
-        for (int sh = 24; sh >= 0; sh -= 8) {
-            for (int i = t; i < 256; i += ST) sm.dig.n[i] = 0, sm.dig.w[i] = 0;
-            __syncthreads();
-            for (int i = t; i < n; i += ST) {
-                const uint32_t k = keys[i];
-                if (!k || k < lim || (sh < 24 && (k >> (sh + 8)) != (prefix >> (sh + 8)))) continue;
-                atomicAdd(&sm.dig.n[(k >> sh) & 255], 1u);
-                if (by_weight && !weightless(k)) atomicAdd(&sm.dig.w[(k >> sh) & 255], weight(k));
-            }
-            __syncthreads();
-            for (int i = t; i < 256; i += ST)
-                if (sm.dig.n[i]) {
-                    atomicAdd(&lead->dig.lead_n[i], sm.dig.n[i]);
-                    if (by_weight) atomicAdd(&lead->dig.lead_w[i], sm.dig.w[i]);
-                }
-            cl.sync();
-            if (rank == 0) {
-                if (t == 0) {
-                    Pick p{0, above_n, 0, above};
-                    int lowest = 0;
-                    while (!sm.dig.lead_n[lowest]) lowest++;
-                    for (int d = 255; d >= lowest; d--) {
-                        if (!sm.dig.lead_n[d]) continue;
-                        const u64 add = by_weight ? sm.dig.lead_w[d] : (u64)sm.dig.lead_n[d];
-                        p.digit = d;
-                        p.ties = sm.dig.lead_n[d];
-                        if (p.above + add >= target || d == lowest) break;  // (the lowest holds the rest)
-                        p.above += add;
-                        p.above_n += p.ties;
-                    }
-                    for (int r = 0; r < C; r++) cl.map_shared_rank(&sm, r)->pick = p;
-                }
-                __syncthreads();
-                for (int i = t; i < 256; i += ST) sm.dig.lead_n[i] = 0, sm.dig.lead_w[i] = 0;
-            }
-            cl.sync();
-            prefix |= (uint32_t)sm.pick.digit << sh;
-            above = sm.pick.above;
-            above_n = sm.pick.above_n;
-            n_tie = sm.pick.ties;
-        }
-        const u64 each = by_weight ? (weightless(prefix) ? 0 : weight(prefix)) : 1, left = target > above ? target - above : 0;
-        u64 m = each ? (left + each - 1) / each : n_tie;
-        if (m < 1) m = 1;
-        if (m > n_tie) m = n_tie;
-        if (prefix == lim && m > lim_ties) m = lim_ties;
-        cut = prefix;
-        ties = (unsigned)m;
-    };
     auto cluster_sum = [&](u64 v, u64 *ahead) {  // over the cluster; *ahead: over the CTAs before this one
         cl.sync();
         if (t < C) cl.map_shared_rank(&sm, t)->total[rank] = v;
         cl.sync();
-        u64 s = 0, pre = 0;
+        u64 sum = 0, pre = 0;
         for (int r = 0; r < C; r++) {
             if (r < rank) pre += sm.total[r];
-            s += sm.total[r];
+            sum += sm.total[r];
         }
         if (ahead) *ahead = pre;
-        return s;
+        return sum;
     };
-    if (k_on) select(false, (u64)top_k, 0, 0xffffffffu);
-    if (p_on) {
-        u64 w = 0, all;
-        for (int i = t; i < n; i += ST)
-            if (keys[i] > cut && !weightless(keys[i])) w += weight(keys[i]);
-        block_scan<u64>(w, sm.scan, lane, warp, &all);
-        all = cluster_sum(all, nullptr);
-        if (cut && !weightless(cut)) all += (u64)ties * weight(cut);
-        select(true, (u64)ceil((double)top_p * (double)all), cut, ties);
-    }
-    // ---- draw in index order: warp w owns indices [w * per, (w + 1) * per) of the slice
+    // warp w owns indices [w * per, (w + 1) * per) of the slice
     const int per = ((n + SW - 1) / SW + 31) & ~31, i0 = min(n, warp * per), i1 = min(n, i0 + per);
-    unsigned tie0 = 0;
-    if (cut) {
-        unsigned mine = 0, all;
-        for (int i = i0 + lane; i < i1; i += 32) mine += keys[i] == cut;
-        mine = __reduce_add_sync(0xffffffffu, mine);
-        const unsigned pre = block_scan<unsigned>(lane == 0 ? mine : 0u, reinterpret_cast<unsigned *>(sm.scan), lane, warp, &all);
-        u64 ahead;
-        cluster_sum(all, &ahead);
-        tie0 = __shfl_sync(0xffffffffu, pre, 0) + (unsigned)ahead;
+    if ((k_on || p_on) && way == RADIX) {
+        // ---- radix selection: most significant digit first, the digit in which
+        // the running count (or weight) from the top reaches the target; of the
+        // tokens from `cut` up. Ends in the last token that stays.
+        auto select = [&](bool by_weight, u64 target) {
+            uint32_t prefix = 0;
+            u64 above = 0;
+            unsigned n_tie = 0;
+            for (int sh = 24; sh >= 0; sh -= 8) {
+                for (int i = t; i < 256; i += ST) sm.dig.n[i] = sm.dig.lead_n[i] = 0, sm.dig.w[i] = sm.dig.lead_w[i] = 0;
+                cl.sync();
+                for (int i = t; i < n; i += ST) {
+                    const uint32_t k = keys[i];
+                    if (!k || token(i) < cut || (sh < 24 && (k >> (sh + 8)) != (prefix >> (sh + 8)))) continue;
+                    atomicAdd(&sm.dig.n[(k >> sh) & 255], 1u);
+                    if (by_weight && !weightless(k)) atomicAdd(&sm.dig.w[(k >> sh) & 255], weight(k));
+                }
+                __syncthreads();
+                for (int i = t; i < 256; i += ST)
+                    if (sm.dig.n[i]) {
+                        atomicAdd(&lead->dig.lead_n[i], sm.dig.n[i]);
+                        if (by_weight) atomicAdd(&lead->dig.lead_w[i], sm.dig.w[i]);
+                    }
+                cl.sync();
+                if (rank == 0) {  // thread t: digit 255 - t
+                    u64 x = 0, all;
+                    unsigned y = 0;
+                    if (t < 256) y = sm.dig.lead_n[255 - t], x = by_weight ? sm.dig.lead_w[255 - t] : (u64)y;
+                    const u64 before = above + block_scan<u64>(x, sm.scan, lane, warp, &all);
+                    if (t == 0) sm.lo = 0, sm.hi = 256;
+                    __syncthreads();
+                    if (y) atomicMax(&sm.lo, t);                                 // the lowest digit holds the rest
+                    if (y && before + x >= target) atomicMin(&sm.hi, t);
+                    __syncthreads();
+                    if (t == min(sm.lo, sm.hi))
+                        for (int r = 0; r < C; r++) cl.map_shared_rank(&sm, r)->pick = Pick{255 - t, y, before};
+                }
+                cl.sync();
+                prefix |= (uint32_t)sm.pick.digit << sh;
+                above = sm.pick.above;
+                n_tie = sm.pick.ties;
+            }
+            const u64 each = by_weight ? (weightless(prefix) ? 0 : weight(prefix)) : 1, left = target > above ? target - above : 0;
+            u64 m = each ? (left + each - 1) / each : n_tie;  // of its ties, by index
+            m = m < 1 ? 1 : m > n_tie ? n_tie : m;
+            // the m-th of them
+            unsigned mine = 0, here;
+            for (int i = i0 + lane; i < i1; i += 32) mine += keys[i] == prefix && token(i) >= cut;
+            mine = __reduce_add_sync(0xffffffffu, mine);
+            unsigned pre = block_scan<unsigned>(lane == 0 ? mine : 0u, reinterpret_cast<unsigned *>(sm.scan), lane, warp, &here);
+            u64 ahead;
+            cluster_sum(here, &ahead);
+            unsigned run = __shfl_sync(0xffffffffu, pre, 0) + (unsigned)ahead;
+            if (run < m && m <= run + mine)
+                for (int i = i0; i < i1; i += 32) {
+                    const bool tie = i + lane < i1 && keys[i + lane] == prefix && token(i + lane) >= cut;
+                    const unsigned same = __ballot_sync(0xffffffffu, tie);
+                    if (tie && run + __popc(same & ((1u << lane) - 1)) + 1 == m)
+                        for (int r = 0; r < C; r++) cl.map_shared_rank(&sm, r)->cut = token(i + lane);
+                    run += __popc(same);
+                }
+            cl.sync();
+            cut = sm.cut;
+        };
+        if (k_on && !cut) select(false, (u64)top_k);
+        if (p_on) {
+            u64 w = 0;
+            for (int i = t; i < n; i += ST)
+                if (!weightless(keys[i]) && token(i) >= cut) w += weight(keys[i]);
+            u64 all;
+            block_scan<u64>(w, sm.scan, lane, warp, &all);
+            all = cluster_sum(all, nullptr);
+            select(true, (u64)ceil((double)top_p * (double)all));
+        }
     }
-    auto kept_weight = [&](int i, unsigned &before) -> u64 {  // of index i, if kept; before: ties ahead of this step
+    // ---- draw in index order from the tokens where they are
+    auto kept_weight = [&](int i) -> u64 {
         const uint32_t k = i < i1 ? keys[i] : 0u;
-        const unsigned same = __ballot_sync(0xffffffffu, k == cut && k);
-        const bool tie = k == cut && before + __popc(same & ((1u << lane) - 1)) < ties;
-        before += __popc(same);
-        if (!k || !(k > cut || tie) || (!first && weightless(k))) return 0;
+        if (!k || token(i) < cut) return 0;
+        if (first) {  // any weight above zero counts 1
+            const double w = k == kmax ? 1.0 : exp(((double)key_logit(k) - lmax) / (double)T);
+            return (u64)(w > 0.0 && !(w < (double)min_p));
+        }
+        if (weightless(k)) return 0;
         const double w = real_weight(k);
-        if (w < floor_w) return 0;
-        return first ? (u64)(w > 0.0) : __double2ull_rn(w * S_ONE);
+        return w < floor_w ? 0 : whole_weight(w);
     };
     u64 sum = 0;
-    unsigned seen = tie0;
-    for (int i = i0; i < i1; i += 32) sum += kept_weight(i + lane, seen);
-    u64 all;
-    const u64 lane_pre = block_scan<u64>(sum, sm.scan, lane, warp, &all);
-    u64 run;
+#pragma unroll 4
+    for (int i = i0; i < i1; i += 32) sum += kept_weight(i + lane);
+    sum = warp_total(sum);
+    u64 all, run;
+    u64 pre = block_scan<u64>(lane == 0 ? sum : 0, sm.scan, lane, warp, &all);
     const u64 total = cluster_sum(all, &run);
-    run += __shfl_sync(0xffffffffu, lane_pre, 0);
-    sum = __shfl_sync(0xffffffffu, lane_pre + sum, 31) - __shfl_sync(0xffffffffu, lane_pre, 0);
+    run += __shfl_sync(0xffffffffu, pre, 0);
     const double x = (double)u * (double)total;
     u64 want = x > 0.0 ? (x < (double)total ? (u64)x : total) : 0;
     if (want >= total) want = total - 1;
     if (run <= want && want < run + sum) {  // this warp holds the token
-        seen = tie0;
         for (int i = i0; i < i1; i += 32) {
-            const u64 w = warp_scan(kept_weight(i + lane, seen), lane);
+            const u64 w = warp_scan(kept_weight(i + lane), lane);
             const unsigned hit = __ballot_sync(0xffffffffu, run + w > want);
             if (hit) {
                 if (lane == 0) a.tokens[out_at] = base + i + __ffs(hit) - 1;
