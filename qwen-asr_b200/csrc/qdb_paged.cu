@@ -29,30 +29,53 @@ __device__ __forceinline__ int row_sequence(const QdbPagedBatch &bt, int row) {
     return lo;
 }
 
-template <typename S>
-__device__ __forceinline__ float load_src(const void *p, size_t i);
 struct SrcF32 {};
-template <>
-__device__ __forceinline__ float load_src<SrcF32>(const void *p, size_t i) {
-    return reinterpret_cast<const float *>(p)[i];
+// 8 consecutive source elements.
+template <typename S>
+__device__ __forceinline__ void load8(const void *p, size_t i, float *v) {
+    const uint4 w = ldg_stream(reinterpret_cast<const uint16_t *>(p) + i);
+    v[0] = S::lo(w.x), v[1] = S::hi(w.x), v[2] = S::lo(w.y), v[3] = S::hi(w.y);
+    v[4] = S::lo(w.z), v[5] = S::hi(w.z), v[6] = S::lo(w.w), v[7] = S::hi(w.w);
 }
 template <>
-__device__ __forceinline__ float load_src<QdbHalf>(const void *p, size_t i) {
-    return QdbHalf::lo(reinterpret_cast<const uint16_t *>(p)[i]);
-}
-template <>
-__device__ __forceinline__ float load_src<QdbBf16>(const void *p, size_t i) {
-    return QdbBf16::lo(reinterpret_cast<const uint16_t *>(p)[i]);
+__device__ __forceinline__ void load8<SrcF32>(const void *p, size_t i, float *v) {
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        const uint4 w = ldg_stream(reinterpret_cast<const float *>(p) + i + 4 * h);
+        v[4 * h] = __uint_as_float(w.x), v[4 * h + 1] = __uint_as_float(w.y);
+        v[4 * h + 2] = __uint_as_float(w.z), v[4 * h + 3] = __uint_as_float(w.w);
+    }
 }
 
-// One warp per (row, head vector).
+// Bound by memory: every row is read once and written once. Eight lanes per
+// head vector: lane i holds dims 8 i .. 8 i + 7 of both halves, the pairs that
+// rotate together, so all loads and stores are 16 bytes. A CTA has 32 vectors
+// of one or several rows; a row's sequence, position and page are looked up
+// once per vector by its own lanes (they hit L1).
+constexpr int AP_THREADS = 256, AP_VECS = AP_THREADS / 8;
+
 template <typename S, typename T>
-__global__ void append_kernel(const QdbAppendArgs a) {
+__global__ void __launch_bounds__(AP_THREADS) append_kernel(const QdbAppendArgs a, int slots) {
     pdl_enter();
-    const int lane = threadIdx.x & 31;
-    const int slot = blockIdx.y * (blockDim.x >> 5) + (threadIdx.x >> 5);
-    const int row = blockIdx.x, Hq = a.heads, Hkv = a.kv.kv_heads;
-    if (slot >= Hq + 2 * Hkv) return;
+    const int i8 = (threadIdx.x & 7) * 8, Hq = a.heads, Hkv = a.kv.kv_heads;
+    const long long vec = (long long)blockIdx.x * AP_VECS + threadIdx.x / 8;
+    const int row = (int)(vec / slots), slot = (int)(vec - (long long)row * slots);
+    const bool here = row < a.bt.rows;
+    // the source does not depend on the look-ups: its loads go first
+    float x[8], y[8];
+    if (here) {
+        const size_t at = (size_t)row * a.row_stride + (size_t)slot * QDB_HD + i8;
+        load8<S>(a.qkv, at, x);
+        load8<S>(a.qkv, at + 64, y);
+    }
+    float ss = 0.f;
+    if (here && slot < Hq + Hkv) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) ss += x[e] * x[e] + y[e] * y[e];
+    }
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    if (!here) return;
     const int b = row_sequence(a.bt, row);
     if (b >= a.bt.n_seqs) return;
     int first, last;
@@ -63,25 +86,27 @@ __global__ void append_kernel(const QdbAppendArgs a) {
     if (pos < 0) return;  // the sequence is shorter than its rows
     // a row that cannot be rotated is left out whole
     if (a.rope && !check_or_record(pos < a.rope_len, a.bt.err, QDB_CHECK_ROPE, b, pos)) return;
-    float e[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) e[i] = load_src<S>(a.qkv, (size_t)row * a.row_stride + slot * QDB_HD + lane + 32 * i);
     if (slot < Hq + Hkv) {
         const float *w = slot < Hq ? a.q_norm : a.k_norm;
         if (w) {
-            const float ss = warp_sum(e[0] * e[0] + e[1] * e[1] + e[2] * e[2] + e[3] * e[3]);
             const float inv = 1.0f / sqrtf(ss / (float)QDB_HD + a.eps);
 #pragma unroll
-            for (int i = 0; i < 4; i++) e[i] = e[i] * inv * w[lane + 32 * i];
+            for (int e = 0; e < 8; e += 4) {
+                const float4 u = *reinterpret_cast<const float4 *>(w + i8 + e), v = *reinterpret_cast<const float4 *>(w + 64 + i8 + e);
+                x[e] *= inv * u.x, x[e + 1] *= inv * u.y, x[e + 2] *= inv * u.z, x[e + 3] *= inv * u.w;
+                y[e] *= inv * v.x, y[e + 1] *= inv * v.y, y[e + 2] *= inv * v.z, y[e + 3] *= inv * v.w;
+            }
         }
         if (a.rope) {
-            const float2 *rr = a.rope + (size_t)pos * (QDB_HD / 2);
+            const float4 *cs = reinterpret_cast<const float4 *>(a.rope + (size_t)pos * (QDB_HD / 2) + i8);
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const float2 cs = rr[lane + 32 * i];
-                const float x1 = e[i], x2 = e[i + 2];
-                e[i] = x1 * cs.x - x2 * cs.y;
-                e[i + 2] = x2 * cs.x + x1 * cs.y;
+            for (int e = 0; e < 8; e += 2) {
+                const float4 r = cs[e / 2];  // (cos, sin) of two pairs
+                const float x0 = x[e], x1 = x[e + 1];
+                x[e] = x0 * r.x - y[e] * r.y;
+                y[e] = y[e] * r.x + x0 * r.y;
+                x[e + 1] = x1 * r.z - y[e + 1] * r.w;
+                y[e + 1] = y[e + 1] * r.z + x1 * r.w;
             }
         }
     }
@@ -96,24 +121,27 @@ __global__ void append_kernel(const QdbAppendArgs a) {
         dst = (is_k ? a.kv.k : a.kv.v) + page * a.kv.page_stride + g * a.kv.head_stride +
               (pos & ((1 << a.kv.page_shift) - 1)) * a.kv.pos_stride;
     }
-#pragma unroll
-    for (int i = 0; i < 4; i++) dst[lane + 32 * i] = T::one(e[i]);
+    *reinterpret_cast<uint4 *>(dst + i8) =
+        make_uint4(T::pack(x[0], x[1]), T::pack(x[2], x[3]), T::pack(x[4], x[5]), T::pack(x[6], x[7]));
+    *reinterpret_cast<uint4 *>(dst + 64 + i8) =
+        make_uint4(T::pack(y[0], y[1]), T::pack(y[2], y[3]), T::pack(y[4], y[5]), T::pack(y[6], y[7]));
 }
 
 }  // namespace
 
-cudaError_t qdb_launch_paged_append(const QdbAppendArgs &a, int src_type, int kv_type, cudaStream_t st) {
+template <typename S>
+static cudaError_t launch_append(const QdbAppendArgs &a, int kv_type, cudaStream_t st) {
     const int slots = a.heads + 2 * a.kv.kv_heads;
-    const dim3 grid(a.bt.rows, (slots + 7) / 8), block(256);
-    const bool h = kv_type == QDB_TYPE_F16;
-    if (src_type == QDB_TYPE_F32)
-        return h ? pdl_launch(append_kernel<SrcF32, QdbHalf>, grid, block, 0, st, a)
-                 : pdl_launch(append_kernel<SrcF32, QdbBf16>, grid, block, 0, st, a);
-    if (src_type == QDB_TYPE_F16)
-        return h ? pdl_launch(append_kernel<QdbHalf, QdbHalf>, grid, block, 0, st, a)
-                 : pdl_launch(append_kernel<QdbHalf, QdbBf16>, grid, block, 0, st, a);
-    return h ? pdl_launch(append_kernel<QdbBf16, QdbHalf>, grid, block, 0, st, a)
-             : pdl_launch(append_kernel<QdbBf16, QdbBf16>, grid, block, 0, st, a);
+    const long long vecs = (long long)a.bt.rows * slots;
+    const dim3 grid((unsigned)((vecs + AP_VECS - 1) / AP_VECS)), block(AP_THREADS);
+    return kv_type == QDB_TYPE_F16 ? pdl_launch(append_kernel<S, QdbHalf>, grid, block, 0, st, a, slots)
+                                   : pdl_launch(append_kernel<S, QdbBf16>, grid, block, 0, st, a, slots);
+}
+
+cudaError_t qdb_launch_paged_append(const QdbAppendArgs &a, int src_type, int kv_type, cudaStream_t st) {
+    if (src_type == QDB_TYPE_F32) return launch_append<SrcF32>(a, kv_type, st);
+    if (src_type == QDB_TYPE_F16) return launch_append<QdbHalf>(a, kv_type, st);
+    return launch_append<QdbBf16>(a, kv_type, st);
 }
 
 cudaError_t qdb_decode_scratch_alloc(int device, QdbDecodeScratch *s) {

@@ -54,12 +54,12 @@ __device__ __forceinline__ float widen(uint32_t bits) {
 // Order-preserving integer of a logit: 0 for NaN and -inf (never drawn); -0
 // and +0 are equal.
 __device__ __forceinline__ uint32_t logit_key(float v) {
-    if (isnan(v) || v == -INFINITY) return 0u;
-    uint32_t b = __float_as_uint(v == 0.f ? 0.f : v);
-    return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+    const uint32_t b = __float_as_uint(v + 0.f);  // (-0 becomes +0)
+    const uint32_t k = b ^ ((uint32_t)((int)b >> 31) | 0x80000000u);
+    return k - 0x00800000u <= 0xff000000u ? k : 0u;  // from the lowest number (0x00800000) to +inf (0xff800000)
 }
 __device__ __forceinline__ float key_logit(uint32_t k) {
-    return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
+    return __uint_as_float(k ^ ((uint32_t)((int)~k >> 31) | 0x80000000u));
 }
 
 template <typename X>
@@ -83,11 +83,10 @@ struct Plan {     // what the CTAs do next: bins lo .. hi go to the list
     int way, lo, hi;
 };
 
-struct SampleSmem {
+struct alignas(16) SampleSmem {
     union {
         struct {
-            unsigned n[BINS];
-            float w[BINS];
+            unsigned n[BINS], f[BINS];  // tokens; their places within the bin, in 1 / 4096, added up
         } hist;
         u64 val[LIST];
     };
@@ -98,13 +97,14 @@ struct SampleSmem {
             unsigned n[256], lead_n[256];
         } dig;
     };
-    double exp2_64[64];  // 2^(45 + i / 64)
+    double exp2_16[16];  // 2^(45 + i / 16): a warp's reads have no bank conflict
     u64 scan[SW + 1];
     float scan_f[SW + 1];
     u64 best[SC], total[SC];
     uint32_t low[SC];
     u64 weight;      // first CTA: a sum of weights
-    unsigned count;  // first CTA: tokens in the list
+    unsigned count;  // tokens in the list
+    unsigned offset;
     u64 cut;         // the last token that stays
     int lo, hi;      // first CTA
     Plan plan;
@@ -128,16 +128,38 @@ __device__ __forceinline__ X block_scan(X v, X *buf, int lane, int warp, X *all)
     return pre + in - v;
 }
 
-// n2 (a power of two) values in descending order.
+// n2 (a power of two, at least 64) values, all different but for zeros, in
+// descending order. Up to 128 by counting the larger ones of each; more by a
+// bitonic network, whose steps over distances up to 32 stay within 64 values of
+// one warp.
 __device__ void sort_down(u64 *x, int n2, int t) {
+    __syncthreads();
+    if (n2 <= 128) {
+        const u64 mine = t < n2 ? x[t] : 0;
+        const int m = __syncthreads_count(mine != 0);
+        int at = 0;
+        if (mine)
+#pragma unroll 8
+            for (int i = 0; i < n2; i += 2) {
+                const ulonglong2 y = *reinterpret_cast<const ulonglong2 *>(x + i);
+                at += (y.x > mine) + (y.y > mine);
+            }
+        __syncthreads();
+        if (mine) x[at] = mine;
+        if (t >= m && t < n2) x[t] = 0;
+        __syncthreads();
+        return;
+    }
     for (int k = 2; k <= n2; k <<= 1)
         for (int j = k >> 1; j > 0; j >>= 1) {
-            __syncthreads();
             for (int p = t; p < n2 / 2; p += ST) {
                 const int i = 2 * p - (p & (j - 1)), q = i + j;
                 const u64 a = x[i], b = x[q];
                 if ((a < b) == ((i & k) == 0)) x[i] = b, x[q] = a;
             }
+            // (the next step is over j / 2, or over k where this one was over 1)
+            if (j > 32 || (j == 1 && k > 32)) __syncthreads();
+            else __syncwarp();
         }
     __syncthreads();
 }
@@ -152,9 +174,9 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const QdbSampleArgs a, in
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5, V = a.vocab;
     const int base = min(V, rank * slice), n = min(V, base + slice) - base;  // this CTA's tokens
     SampleSmem *lead = cl.map_shared_rank(&sm, 0);
-    for (int i = t; i < BINS; i += ST) sm.hist.n[i] = 0, sm.hist.w[i] = 0.f;
+    for (int i = t; i < BINS; i += ST) sm.hist.n[i] = 0, sm.hist.f[i] = 0;
     if (t == 0) sm.weight = 0, sm.count = 0;
-    if (t < 64) sm.exp2_64[t] = exp2(45.0 + t / 64.0);
+    if (t < 16) sm.exp2_16[t] = exp2(45.0 + t / 16.0);
     cl.barrier_arrive();  // (waited for before the first access to another CTA's memory)
     pdl_enter();
     const size_t out_at = (a.step ? (size_t)*a.step * a.rows : 0) + row;
@@ -164,32 +186,57 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const QdbSampleArgs a, in
     const float u = a.uniform[out_at];
 
     // ---- 1. the row into shared memory; its maximum
+    // (thread t has tokens 4 t .. 4 t + 3, those 4 ST further on, and so on)
     u64 best = 0;
-    uint32_t low = 0xffffffffu;
+    uint32_t bk = 0, bi = 0;      // this thread's largest key, its first place
+    uint32_t low = 0xffffffffu;   // smallest key above 0, less 1
     {
-        constexpr int ES = TYPE == QDB_TYPE_F32 ? 4 : 2, PER = 16 / ES;
+        constexpr int ES = TYPE == QDB_TYPE_F32 ? 4 : 2;
         const char *src = (const char *)a.logits + ((size_t)row * a.row_stride + base) * ES;
-        auto put = [&](int i, uint32_t bits) {
-            uint32_t k = logit_key(widen<TYPE>(bits));
-            if (a.mask_eos && (base + i == QDB_ENDOFTEXT || base + i == QDB_IM_END)) k = 0;
-            keys[i] = k;
-            const u64 c = (u64)k << 32 | (0xffffffffu - (uint32_t)(base + i));
-            if (k) best = c > best ? c : best, low = min(low, k);
-        };
-        int from = 0;
-        if (((uintptr_t)src & 15) == 0) {
-            from = n / PER * PER;
-#pragma unroll 4
-            for (int i = t * PER; i < from; i += ST * PER) {
-                const uint4 x = ldg_stream(src + (size_t)i * ES);
-                const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+        const bool vec = ((uintptr_t)src & (4 * ES - 1)) == 0;
+        constexpr int B = 4;  // loads in flight
+        for (int i = t * 4; i < n; i += B * ST * 4) {
+            uint4 x[B];
 #pragma unroll
-                for (int e = 0; e < PER; e++) put(i + e, ES == 4 ? w[e] : (w[e / 2] >> (16 * (e & 1))) & 0xffffu);
+            for (int e = 0; e < B; e++) {
+                const int j = i + e * ST * 4;
+                const char *at = src + (size_t)j * ES;
+                if (vec && j + 4 <= n) {
+                    if (ES == 4) {
+                        x[e] = ldg_stream(at);
+                    } else {
+                        const uint2 y = *reinterpret_cast<const uint2 *>(at);
+                        x[e] = make_uint4(y.x & 0xffffu, y.x >> 16, y.y & 0xffffu, y.y >> 16);
+                    }
+                } else {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int f = 0; f < 4; f++)
+                        w[f] = j + f >= n ? (TYPE == QDB_TYPE_F32 ? 0xff800000u : TYPE == QDB_TYPE_F16 ? 0xfc00u : 0xff80u)
+                               : ES == 4  ? reinterpret_cast<const uint32_t *>(src)[j + f]
+                                          : (uint32_t) reinterpret_cast<const uint16_t *>(src)[j + f];  // (-inf behind the end)
+                    x[e] = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < B; e++) {
+                const int j = i + e * ST * 4;
+                if (j >= n) break;
+                uint32_t k[4] = {logit_key(widen<TYPE>(x[e].x)), logit_key(widen<TYPE>(x[e].y)),
+                                 logit_key(widen<TYPE>(x[e].z)), logit_key(widen<TYPE>(x[e].w))};
+                if (a.mask_eos)
+#pragma unroll
+                    for (int f = 0; f < 4; f++)
+                        if (base + j + f == QDB_ENDOFTEXT || base + j + f == QDB_IM_END) k[f] = 0;
+#pragma unroll
+                for (int f = 0; f < 4; f++) {
+                    if (k[f] > bk) bk = k[f], bi = j + f;
+                    low = min(low, k[f] - 1);  // (0 wraps round: not counted)
+                }
+                *reinterpret_cast<uint4 *>(keys + j) = make_uint4(k[0], k[1], k[2], k[3]);
             }
         }
-#pragma unroll 4
-        for (int i = from + t; i < n; i += ST)
-            put(i, ES == 4 ? reinterpret_cast<const uint32_t *>(src)[i] : (uint32_t) reinterpret_cast<const uint16_t *>(src)[i]);
+        if (bk) best = (u64)bk << 32 | (0xffffffffu - (uint32_t)(base + bi));
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -220,29 +267,45 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const QdbSampleArgs a, in
     }
     const uint32_t kmax = (uint32_t)(best >> 32);
     const float fmax = key_logit(kmax);
-    const double lmax = (double)fmax, floor_w = (double)min_p * S_ONE;
+    const bool top_inf = isinf(fmax);  // (then only tokens that share it weigh)
+    const double lmax = top_inf ? 0.0 : (double)fmax;
     const bool k_on = top_k > 0 && top_k < V, p_on = top_p < 1.f, first = !(u > 0.f);
-    // 2^45 exp((l - max) / T) by 2^(i / 64) from the table times a polynomial of
-    // degree 4 in the rest (below 0.0055: the next term is 2^-44 of the weight)
-    const double c64 = 64.0 * 1.4426950408889634074 / (double)T;
-    auto real_weight = [&](uint32_t k) -> double {
-        if (k == kmax) return S_ONE;
-        const double d = (double)key_logit(k) - lmax, magic = 6755399441055744.0;  // 1.5 * 2^52
-        const double y = fma(d, c64, magic);
+    // 2^45 exp((l - max) / T) = 2^45 2^(y / 16) by 2^(i / 16) from the table times a
+    // polynomial of degree 5 in x = y - i, |x| <= 1/2 (the next term is below 2^-42)
+    const double c16 = 16.0 * 1.4426950408889634074 / (double)T;
+    constexpr double E1 = 0.69314718055994530942 / 16, E2 = E1 * E1 / 2, E3 = E2 * E1 / 3, E4 = E3 * E1 / 4, E5 = E4 * E1 / 5;
+    // keys below `least` (logits more than `reach` below the maximum) weigh
+    // nothing; with an infinite maximum only those that share it weigh
+    const float reach = S_REACH * T, bottom = fmax - reach;
+    const uint32_t least = isnan(bottom) ? kmax : max(1u, min(kmax, logit_key(bottom)));
+    auto weightless = [&](uint32_t k) { return k < least; };
+    auto real_weight = [&](uint32_t k) -> double {  // without a branch: 0 where it is weightless
+        const double d = (double)(top_inf ? 0.f : key_logit(k)) - lmax, magic = 6755399441055744.0;  // 1.5 * 2^52
+        const double y = fma(d, c16, magic);
         const int i = __double2loint(y);
-        const double x = fma(d, c64, magic - y) * (0.69314718055994530942 / 64.0);
-        double e = fma(x, 1.0 / 24, 1.0 / 6);
-        e = fma(x, e, 0.5);
-        e = fma(x, e, 1.0);
-        e = fma(x, e, 1.0) * sm.exp2_64[i & 63];
-        return __hiloint2double(__double2hiint(e) + ((i >> 6) << 20), __double2loint(e));
+        const double x = fma(d, c16, magic - y);
+        double e = fma(x, E5, E4);
+        e = fma(x, e, E3);
+        e = fma(x, e, E2);
+        e = fma(x, e, E1);
+        e = fma(x, e, 1.0) * sm.exp2_16[i & 15];
+        e = __hiloint2double(__double2hiint(e) + ((i >> 4) << 20), __double2loint(e));
+        return weightless(k) ? 0.0 : e;
     };
     auto whole_weight = [&](double w) -> u64 {  // rounded to an integer (below 2^51)
         return (u64)__double_as_longlong(w + 4503599627370496.0) & ((1ull << 52) - 1);
     };
     auto weight = [&](uint32_t k) { return whole_weight(real_weight(k)); };
-    const float reach = S_REACH * T;  // logits further below the maximum weigh nothing
-    auto weightless = [&](uint32_t k) { return !k || (k != kmax && !(fmax - key_logit(k) <= reach)); };
+    // Calls f(i, k) for this CTA's tokens i .. i + 3 with keys k[4], whose
+    // arithmetic then overlaps (0 behind the end).
+    auto each4 = [&](auto f) {
+        for (int i = t * 4; i < n; i += ST * 4) {
+            const uint4 x = *reinterpret_cast<const uint4 *>(keys + i);
+            const uint32_t k[4] = {x.x, x.y, x.z, x.w};
+            f(i, k);
+        }
+    };
+    auto token_of = [&](uint32_t k, int i) { return (u64)k << 32 | (0xffffffffu - (uint32_t)(base + i)); };
     auto token = [&](int i) { return (u64)keys[i] << 32 | (0xffffffffu - (uint32_t)(base + i)); };
     auto warp_total = [&](u64 v) {
 #pragma unroll
@@ -250,106 +313,274 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const QdbSampleArgs a, in
         return v;
     };
     // Tokens that `take` wants to the first CTA's list (in any order); a
-    // barrier of the cluster has to follow.
-    auto gather = [&](auto take) {
-        for (int i0 = warp * 32; i0 < n; i0 += ST) {
-            const bool yes = i0 + lane < n && take(i0 + lane);
-            const unsigned m = __ballot_sync(0xffffffffu, yes);
-            if (!m) continue;
-            unsigned at = 0;
-            if (lane == 0) at = atomicAdd(&lead->count, __popc(m));
-            at = __shfl_sync(0xffffffffu, at, 0) + __popc(m & ((1u << lane) - 1));
-            if (yes && at < LIST) lead->list[at] = token(i0 + lane);
+    // barrier of the cluster has to follow. Each CTA collects in its own list.
+    auto gather = [&](uint32_t from, auto take) {
+        if (rank) {
+            __syncthreads();
+            if (t == 0) sm.count = 0;
+            __syncthreads();
+        }
+        if (bk >= from)  // (else this thread has no key from there on)
+        each4([&](int i, const uint32_t *k) {
+            bool yes[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) yes[e] = take(k[e], i + e);
+            if (!(yes[0] | yes[1] | yes[2] | yes[3])) return;
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (yes[e]) {
+                    const unsigned at = atomicAdd(&sm.count, 1u);
+                    if (at < LIST) sm.list[at] = token_of(k[e], i + e);
+                }
+        });
+        if (rank) {
+            __syncthreads();
+            if (t == 0) sm.offset = atomicAdd(&lead->count, sm.count);
+            __syncthreads();
+            const unsigned at = sm.offset;
+            for (int i = t; i < (int)min(sm.count, (unsigned)LIST); i += ST)
+                if (at + i < LIST) lead->list[at + i] = sm.list[i];
         }
     };
     // First CTA: sorts the list; returns its length.
     auto sort_list = [&](int *n2) {
         const int m = min((int)sm.count, LIST);
-        *n2 = 32;
+        *n2 = 64;
         while (*n2 < m) *n2 <<= 1;
         for (int i = m + t; i < *n2; i += ST) sm.list[i] = 0;
         sort_down(sm.list, *n2, t);
         return m;
     };
     constexpr int PT = BINS / ST;  // bins, or list entries, of a thread
-    u64 cut = 0;                   // tokens from here up stay
+    u64 cut = 0, min_cut = 0;      // tokens from here up stay (by top_k and top_p, by min_p)
     int way = RADIX;
 
     // ---- 2. histogram: how far down the kept tokens can go
-    const float span = fminf(reach, fmax - key_logit(low)), s = span > 0.f ? (float)BINS / span : 0.f;
-    auto bin_of = [&](uint32_t k) { return k == kmax ? 0 : min(BINS - 1, (int)((fmax - key_logit(k)) * s)); };
+    const float span = fminf(reach, fmax - key_logit(low + 1)), s = span > 0.f ? BINS * 4096.f / span : 0.f;
+    auto place_of = [&](uint32_t k) { return min(BINS * 4096 - 1, (int)((fmax - key_logit(k)) * s)); };
+    auto bin_of = [&](uint32_t k) { return place_of(k) >> 12; };
+    // The smallest key from `least` on that `in` holds for (it holds for larger
+    // ones and for kmax), found by the warp 32 at a time.
+    auto first_key = [&](auto in) {
+        uint32_t lo = least, width = kmax - least + 1;  // the key is in [lo, lo + width)
+        while (width > 1) {
+            const uint32_t step = (width + 31) / 32;
+            const u64 end = (u64)(lane + 1) * step;  // lane's group: does its last key qualify?
+            const bool yes = end >= width || in(lo + (uint32_t)end - 1);
+            const uint32_t g = __ffs(__ballot_sync(0xffffffffu, yes)) - 1;
+            lo += g * step;
+            width = min(step, width - g * step);
+        }
+        return lo;
+    };
+    auto bin_start = [&](int bin) { return first_key([&](uint32_t k) { return bin_of(k) <= bin; }); };
+    // min_p as a cut
+    if (min_p > 0.f && !first) {
+        const double floor_w = (double)min_p * S_ONE;
+        min_cut = (u64)first_key([&](uint32_t k) { return real_weight(k) >= floor_w; }) << 32;
+    }
+    // warp w owns indices [w * per, (w + 1) * per) of the slice
+    const int per = ((n + SW - 1) / SW + 127) & ~127, i0 = min(n, warp * per), i1 = min(n, i0 + per);
+    // The weight of this warp's tokens that `take` wants (weights are computed
+    // only where some lane has one).
+    auto range_sum = [&](auto take) {
+        u64 sum = 0;
+        for (int i = i0 + lane * 4; i - lane * 4 < i1; i += 128) {
+            uint4 x = make_uint4(0u, 0u, 0u, 0u);
+            if (i < i1) x = *reinterpret_cast<const uint4 *>(keys + i);
+            const uint32_t k[4] = {x.x, x.y, x.z, x.w};
+            bool yes[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) yes[e] = take(k[e], i + e);
+            if (!__any_sync(0xffffffffu, yes[0] | yes[1] | yes[2] | yes[3])) continue;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const u64 w = weight(k[e]);
+                sum += yes[e] ? w : 0;
+            }
+        }
+        return warp_total(sum);
+    };
+    u64 range = 0;           // of the tokens that stay, if known
+    bool have_range = false;
+    // ---- 3. First CTA: cuts the list exactly, sorts what stays by index and
+    // draws.
+    auto draw_listed = [&] {
+        int n2;
+        const int m = sort_list(&n2);
+        // (logit descending, index ascending): thread t has entries t * PT ..
+        u64 w[PT], mine = 0, total;
+#pragma unroll
+        for (int e = 0; e < PT; e++) {
+            const int i = t * PT + e;
+            w[e] = i < m && (!k_on || i < top_k) ? weight((uint32_t)(sm.list[i] >> 32)) : 0;
+            mine += w[e];
+        }
+        u64 before = block_scan<u64>(mine, sm.scan, lane, warp, &total);
+        const u64 whole = k_on ? total : sm.weight;
+        const u64 goal = p_on ? (u64)ceil((double)top_p * (double)whole) : ~0ull;
+        // kept ones as index << 46 | weight (at most 2^45), in ascending order
+        // of the index: complemented for the descending sort
+#pragma unroll
+        for (int e = 0; e < PT; e++) {
+            const int i = t * PT + e;
+            u64 x = 0;
+            if (w[e] && before < goal) {
+                const u64 c = sm.list[i];
+                if (c >= min_cut) x = ~((u64)(0xffffffffu - (uint32_t)c) << 46 | w[e]);
+            }
+            before += w[e];
+            if (i < n2) sm.val[i] = x;
+        }
+        sort_down(sm.val, n2, t);
+        mine = 0;
+#pragma unroll
+        for (int e = 0; e < PT; e++) {
+            const u64 x = t * PT + e < n2 ? sm.val[t * PT + e] : 0;
+            w[e] = x ? ~x & ((1ull << 46) - 1) : 0;
+            mine += w[e];
+        }
+        before = block_scan<u64>(mine, sm.scan, lane, warp, &total);
+        const double x = (double)u * (double)total;
+        u64 want = x < (double)total ? (u64)x : total;
+        if (want >= total) want = total - 1;
+#pragma unroll
+        for (int e = 0; e < PT; e++) {
+            if (w[e] && before <= want && want < before + w[e]) a.tokens[out_at] = (int)(~sm.val[t * PT + e] >> 46);
+            before += w[e];
+        }
+    };
+    unsigned cn = 0, all_n;  // first CTA: tokens and (in f32) weight ahead of this thread's bins
+    float cw = 0.f, all_w;
+    // First CTA: adds up the cluster's histograms. A bin's weight is taken as its
+    // tokens times the weight at their mean place: off by less than 2^-14, since
+    // weights within a bin differ by at most a factor of 1.016.
+    float bin_w[PT];
+    auto collect = [&](bool weights) {
+        static_assert(PT == 4, "a thread's bins are one vector");
+        uint4 bn = reinterpret_cast<const uint4 *>(sm.hist.n)[t], bf = reinterpret_cast<const uint4 *>(sm.hist.f)[t];
+#pragma unroll
+        for (int r = 1; r < SC; r++)
+            if (r < C) {
+                const SampleSmem *o = cl.map_shared_rank(&sm, r);
+                const uint4 y = reinterpret_cast<const uint4 *>(o->hist.n)[t];
+                bn.x += y.x, bn.y += y.y, bn.z += y.z, bn.w += y.w;
+                if (weights) {
+                    const uint4 z = reinterpret_cast<const uint4 *>(o->hist.f)[t];
+                    bf.x += z.x, bf.y += z.y, bf.z += z.z, bf.w += z.w;
+                }
+            }
+        reinterpret_cast<uint4 *>(sm.hist.n)[t] = bn;
+        cn = block_scan<unsigned>(bn.x + bn.y + bn.z + bn.w, reinterpret_cast<unsigned *>(sm.scan), lane, warp, &all_n);
+        if (weights) {
+            const unsigned cnt[PT] = {bn.x, bn.y, bn.z, bn.w}, pl[PT] = {bf.x, bf.y, bf.z, bf.w};
+            const float c = s > 0.f ? -1.4426950408889634f / T / s * 4096.f : 0.f;  // log2 of the weight per bin
+            float w = 0.f;
+#pragma unroll
+            for (int e = 0; e < PT; e++) {
+                const float at = (float)(t * PT + e) + (cnt[e] ? (float)pl[e] / ((float)cnt[e] * 4096.f) : 0.f);
+                bin_w[e] = cnt[e] ? (float)cnt[e] * exp2f(at * c) : 0.f;
+                w += bin_w[e];
+            }
+            cw = block_scan<float>(w, sm.scan_f, lane, warp, &all_w);
+        }
+    };
+    // First CTA: sm.hi = the bin in which the count reaches top_k (or the last one).
+    auto k_bin = [&] {
+        int lim = BINS - 1;
+        unsigned x = cn;
+#pragma unroll
+        for (int e = 0; e < PT; e++) {
+            x += sm.hist.n[t * PT + e];
+            if (lim == BINS - 1 && x >= (unsigned)top_k) lim = t * PT + e;
+        }
+        if (t == 0) sm.hi = BINS - 1;
+        __syncthreads();
+        lim = __reduce_min_sync(0xffffffffu, lim);
+        if (lane == 0) atomicMin(&sm.hi, lim);
+        __syncthreads();
+    };
+    // First CTA: `way` and its bins to every CTA.
+    auto tell = [&](int way, int lo, int hi) {
+        if (t < C) cl.map_shared_rank(&sm, t)->plan = Plan{way, lo, hi};
+    };
+    // A top_k that is small beside the number of threads: the top_k-th largest of
+    // the threads' largest keys is a lower bound of the top_k-th key, and few
+    // tokens lie above it.
+    if (k_on && !first && top_k <= C * ST / 4) {
+        if (bk >= least) atomicAdd(&sm.hist.n[bin_of(bk)], 1u);
+        cl.sync();
+        if (rank == 0) {
+            collect(false);
+            k_bin();
+            tell(ALL_LISTED, 0, sm.hi);
+        }
+        cl.sync();
+        const uint32_t from = bin_start(sm.plan.hi);
+        gather(from, [&](uint32_t k, int) { return k >= from; });
+        cl.sync();
+        const bool fits = lead->count <= LIST;
+        cl.barrier_arrive();
+        if (fits && rank == 0) draw_listed();
+        cl.barrier_wait();  // (nobody leaves while the first CTA's count may be read)
+        if (fits) return;
+        // many equal logits: start again with all tokens counted
+        for (int i = t; i < BINS; i += ST) sm.hist.n[i] = 0, sm.hist.f[i] = 0;
+        if (t == 0) sm.count = 0;
+        cl.sync();
+    }
     if ((k_on || p_on) && !first) {
         const bool need_w = p_on && (!k_on || top_k > LIST);
         u64 sum = 0;
-        const float c = -1.4426950408889634f / T;
-#pragma unroll 4
-        for (int i = t; i < n; i += ST) {
-            const uint32_t k = keys[i];
-            if (weightless(k)) continue;
-            const int b = bin_of(k);
-            atomicAdd(&sm.hist.n[b], 1u);
-            if (need_w) {
-                atomicAdd(&sm.hist.w[b], k == kmax ? 1.f : exp2f((fmax - key_logit(k)) * c));
-                if (!k_on) sum += weight(k);
+        each4([&](int, const uint32_t *k) {
+            int b[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                b[e] = place_of(k[e]);
+                b[e] = weightless(k[e]) ? -1 : b[e];
             }
-        }
+            if (need_w && !k_on)
+#pragma unroll
+                for (int e = 0; e < 4; e++) sum += weight(k[e]);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                if (b[e] < 0) continue;
+                atomicAdd(&sm.hist.n[b[e] >> 12], 1u);
+                if (need_w) atomicAdd(&sm.hist.f[b[e] >> 12], (unsigned)b[e] & 4095u);
+            }
+        });
         if (p_on && !k_on) {
             sum = warp_total(sum);
             if (lane == 0) atomicAdd(&lead->weight, sum);
         }
-        __syncthreads();
-        if (rank)
-            for (int i = t; i < BINS; i += ST)
-                if (sm.hist.n[i]) {
-                    atomicAdd(&lead->hist.n[i], sm.hist.n[i]);
-                    if (need_w) atomicAdd(&lead->hist.w[i], sm.hist.w[i]);
-                }
         cl.sync();
-        unsigned cn = 0, all_n;  // first CTA: tokens and (in f32) weight ahead of this thread's bins
-        float cw = 0.f, all_w;
         // First CTA: bins lo .. hi that hold the end of the top_p for a given
-        // total weight. The f32 sums are taken to be off by up to 2^-11 (more only
-        // where bins hold thousands of tokens: what was found is checked).
+        // total weight. The f32 weights are taken to be off by up to 2^-11 (what was
+        // found is checked).
         auto p_bins = [&](u64 whole) {
             const float goal = (float)((double)top_p * (double)whole / S_ONE);
             float w = cw;
             int lo = BINS - 1, hi = BINS - 1;
 #pragma unroll
-            for (int e = PT - 1; e >= 0; e--) {
-                float x = w;
-                for (int f = 0; f <= e; f++) x += sm.hist.w[t * PT + f];
-                if (x * (1.f + 1.f / 2048) >= goal) lo = t * PT + e;
-                if (x * (1.f - 1.f / 2048) >= goal) hi = t * PT + e;
+            for (int e = 0; e < PT; e++) {
+                w += bin_w[e];
+                if (lo == BINS - 1 && w * (1.f + 1.f / 2048) >= goal) lo = t * PT + e;
+                if (hi == BINS - 1 && w * (1.f - 1.f / 2048) >= goal) hi = t * PT + e;
             }
             if (t == 0) sm.lo = sm.hi = BINS - 1;
             __syncthreads();
-            atomicMin(&sm.lo, lo);
-            atomicMin(&sm.hi, hi);
+            lo = __reduce_min_sync(0xffffffffu, lo);
+            hi = __reduce_min_sync(0xffffffffu, hi);
+            if (lane == 0) {
+                atomicMin(&sm.lo, lo);
+                atomicMin(&sm.hi, hi);
+            }
             __syncthreads();
         };
-        auto tell = [&](int way, int lo, int hi) {  // first CTA
-            if (t < C) cl.map_shared_rank(&sm, t)->plan = Plan{way, lo, hi};
-        };
         if (rank == 0) {
-#pragma unroll
-            for (int e = 0; e < PT; e++) cn += sm.hist.n[t * PT + e], cw += sm.hist.w[t * PT + e];
-            cn = block_scan<unsigned>(cn, reinterpret_cast<unsigned *>(sm.scan), lane, warp, &all_n);
-            cw = block_scan<float>(cw, sm.scan_f, lane, warp, &all_w);
-            if (k_on) {  // the bin in which the count is reached
-                int lim = BINS - 1;
-                unsigned x = cn;
-#pragma unroll
-                for (int e = 0; e < PT; e++) {
-                    x += sm.hist.n[t * PT + e];
-                    if (lim == BINS - 1 && x >= (unsigned)top_k) lim = t * PT + e;
-                }
-                if (t == 0) sm.hi = BINS - 1;
-                __syncthreads();
-                atomicMin(&sm.hi, lim);
-                __syncthreads();
-            } else {
-                p_bins(sm.weight);
-            }
+            collect(need_w);
+            if (k_on) k_bin();
+            else p_bins(sm.weight);
             // tokens down to hi, and in lo .. hi
             const int hi = sm.hi, lo = k_on ? hi : sm.lo;
             auto upto = [&](int bin, unsigned *dst) {
@@ -372,8 +603,8 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const QdbSampleArgs a, in
         cl.sync();
         way = sm.plan.way;
         if (way == K_BIN) {  // the end of the top_k
-            const int bin = sm.plan.hi;
-            gather([&](int i) { return !weightless(keys[i]) && bin_of(keys[i]) == bin; });
+            const uint32_t from = bin_start(sm.plan.hi), to = sm.plan.hi ? bin_start(sm.plan.hi - 1) : kmax + 1;
+            gather(from, [&](uint32_t k, int) { return (k >= from) & (k < to); });
             cl.sync();
             if (rank == 0) {
                 int n2;
@@ -389,8 +620,10 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const QdbSampleArgs a, in
                 way = ALL_LISTED;
             } else if (p_on) {  // the weight of the top_k, then the bins of the top_p
                 u64 w = 0;
-                for (int i = t; i < n; i += ST)
-                    if (!weightless(keys[i]) && token(i) >= cut) w += weight(keys[i]);
+                each4([&](int i, const uint32_t *k) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) w += token_of(k[e], i + e) >= cut ? weight(k[e]) : 0;
+                });
                 w = warp_total(w);
                 if (lane == 0) atomicAdd(&lead->weight, w);
                 cl.sync();
@@ -403,22 +636,13 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const QdbSampleArgs a, in
             }
         }
         if (way == P_BINS) {  // the end of the top_p
-            const int lo = sm.plan.lo, hi = sm.plan.hi;
-            u64 w = 0;
-#pragma unroll 2
-            for (int i = t; i < n; i += ST) {
-                const uint32_t k = keys[i];
-                if (!weightless(k) && bin_of(k) < lo && token(i) >= cut) w += weight(k);
-            }
-            w = warp_total(w);
+            // keys from .. to - 1 are in bins lo .. hi
+            const uint32_t from = bin_start(sm.plan.hi), to = sm.plan.lo ? bin_start(sm.plan.lo - 1) : kmax + 1;
+            const u64 w = range_sum([&](uint32_t k, int i) { return (k >= to) & (token_of(k, i) >= cut); });
             if (t == 0 && rank == 0) sm.total[0] = 0;
             cl.sync();
             if (lane == 0) atomicAdd(&lead->total[0], w);
-            gather([&](int i) {
-                if (weightless(keys[i]) || token(i) < cut) return false;
-                const int b = bin_of(keys[i]);
-                return b >= lo && b <= hi;
-            });
+            gather(from, [&](uint32_t k, int i) { return (k >= from) & (k < to) & (token_of(k, i) >= cut); });
             cl.sync();
             if (rank == 0) {
                 int n2;
@@ -449,57 +673,21 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const QdbSampleArgs a, in
             }
             cl.sync();
             way = sm.plan.way;
-            if (way == P_BINS) cut = sm.cut;
+            if (way == P_BINS) {
+                cut = sm.cut;
+                if (min_cut <= (u64)to << 32) {  // the sum goes on with the last bins' tokens
+                    range = w + range_sum([&](uint32_t k, int i) {
+                        return (k < to) & (token_of(k, i) >= cut) & (token_of(k, i) >= min_cut);
+                    });
+                    have_range = true;
+                }
+            }
         }
         if (way == ALL_LISTED) {
-            // ---- 3. the tokens that may stay to the first CTA
-            const int hi = sm.plan.hi;
-            gather([&](int i) { return !weightless(keys[i]) && (cut ? token(i) >= cut : bin_of(keys[i]) <= hi); });
+            const uint32_t from = cut ? least : bin_start(sm.plan.hi);
+            gather(from, [&](uint32_t k, int i) { return (k >= from) & (token_of(k, i) >= cut); });
             cl.sync();
-            if (rank) return;
-            int n2;
-            const int m = sort_list(&n2);
-            // (logit descending, index ascending): thread t has entries t * PT ..
-            u64 w[PT], mine = 0, total;
-#pragma unroll
-            for (int e = 0; e < PT; e++) {
-                const int i = t * PT + e;
-                w[e] = i < m && (!k_on || i < top_k) ? weight((uint32_t)(sm.list[i] >> 32)) : 0;
-                mine += w[e];
-            }
-            u64 before = block_scan<u64>(mine, sm.scan, lane, warp, &total);
-            const u64 whole = k_on ? total : sm.weight;
-            const u64 goal = p_on ? (u64)ceil((double)top_p * (double)whole) : ~0ull;
-            // kept ones as index << 46 | weight (at most 2^45), in ascending order
-            // of the index: complemented for the descending sort
-#pragma unroll
-            for (int e = 0; e < PT; e++) {
-                const int i = t * PT + e;
-                u64 x = 0;
-                if (w[e] && before < goal) {
-                    const u64 c = sm.list[i];
-                    if (!(real_weight((uint32_t)(c >> 32)) < floor_w)) x = ~((u64)(0xffffffffu - (uint32_t)c) << 46 | w[e]);
-                }
-                before += w[e];
-                if (i < n2) sm.val[i] = x;
-            }
-            sort_down(sm.val, n2, t);
-            mine = 0;
-#pragma unroll
-            for (int e = 0; e < PT; e++) {
-                const u64 x = t * PT + e < n2 ? sm.val[t * PT + e] : 0;
-                w[e] = x ? ~x & ((1ull << 46) - 1) : 0;
-                mine += w[e];
-            }
-            before = block_scan<u64>(mine, sm.scan, lane, warp, &total);
-            const double x = (double)u * (double)total;
-            u64 want = x < (double)total ? (u64)x : total;
-            if (want >= total) want = total - 1;
-#pragma unroll
-            for (int e = 0; e < PT; e++) {
-                if (w[e] && before <= want && want < before + w[e]) a.tokens[out_at] = (int)(~sm.val[t * PT + e] >> 46);
-                before += w[e];
-            }
+            if (rank == 0) draw_listed();
             return;
         }
     }
@@ -516,8 +704,6 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const QdbSampleArgs a, in
         if (ahead) *ahead = pre;
         return sum;
     };
-    // warp w owns indices [w * per, (w + 1) * per) of the slice
-    const int per = ((n + SW - 1) / SW + 31) & ~31, i0 = min(n, warp * per), i1 = min(n, i0 + per);
     if ((k_on || p_on) && way == RADIX) {
         // ---- radix selection: most significant digit first, the digit in which
         // the running count (or weight) from the top reaches the target; of the
@@ -594,21 +780,31 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const QdbSampleArgs a, in
         }
     }
     // ---- draw in index order from the tokens where they are
-    auto kept_weight = [&](int i) -> u64 {
-        const uint32_t k = i < i1 ? keys[i] : 0u;
-        if (!k || token(i) < cut) return 0;
+    cut = cut > min_cut ? cut : min_cut;
+    auto kept_weight = [&](uint32_t k, int i) -> u64 {
         if (first) {  // any weight above zero counts 1
-            const double w = k == kmax ? 1.0 : exp(((double)key_logit(k) - lmax) / (double)T);
+            if (!k || token_of(k, i) < cut) return 0;
+            const double w = k == kmax ? 1.0 : top_inf ? 0.0 : exp(((double)key_logit(k) - lmax) / (double)T);
             return (u64)(w > 0.0 && !(w < (double)min_p));
         }
-        if (weightless(k)) return 0;
-        const double w = real_weight(k);
-        return w < floor_w ? 0 : whole_weight(w);
+        return token_of(k, i) < cut ? 0 : weight(k);
     };
-    u64 sum = 0;
-#pragma unroll 4
-    for (int i = i0; i < i1; i += 32) sum += kept_weight(i + lane);
-    sum = warp_total(sum);
+    auto four = [&](int i, u64 *w) {  // of tokens i .. i + 3 of this warp's range; returns their sum
+        uint4 x = make_uint4(0u, 0u, 0u, 0u);
+        if (i < i1) x = *reinterpret_cast<const uint4 *>(keys + i);
+        w[0] = kept_weight(x.x, i);
+        w[1] = kept_weight(x.y, i + 1);
+        w[2] = kept_weight(x.z, i + 2);
+        w[3] = kept_weight(x.w, i + 3);
+        return (w[0] + w[1]) + (w[2] + w[3]);
+    };
+    u64 sum = range, w[4];
+    if (first) {
+        for (int i = i0; i < i1; i += 128) sum += four(i + lane * 4, w);
+        sum = warp_total(sum);
+    } else if (!have_range) {
+        sum = range_sum([&](uint32_t k, int i) { return (k >= least) & (token_of(k, i) >= cut); });
+    }
     u64 all, run;
     u64 pre = block_scan<u64>(lane == 0 ? sum : 0, sm.scan, lane, warp, &all);
     const u64 total = cluster_sum(all, &run);
@@ -617,14 +813,19 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const QdbSampleArgs a, in
     u64 want = x > 0.0 ? (x < (double)total ? (u64)x : total) : 0;
     if (want >= total) want = total - 1;
     if (run <= want && want < run + sum) {  // this warp holds the token
-        for (int i = i0; i < i1; i += 32) {
-            const u64 w = warp_scan(kept_weight(i + lane), lane);
-            const unsigned hit = __ballot_sync(0xffffffffu, run + w > want);
+        for (int i = i0; i < i1; i += 128) {
+            const u64 mine = four(i + lane * 4, w), upto = run + warp_scan(mine, lane);
+            const unsigned hit = __ballot_sync(0xffffffffu, upto > want);
             if (hit) {
-                if (lane == 0) a.tokens[out_at] = base + i + __ffs(hit) - 1;
+                if (lane == __ffs(hit) - 1) {
+                    u64 at = upto - mine;
+                    int e = 0;
+                    while (e < 3 && (at += w[e]) <= want) e++;
+                    a.tokens[out_at] = base + i + lane * 4 + e;
+                }
                 break;
             }
-            run += __shfl_sync(0xffffffffu, w, 31);
+            run = __shfl_sync(0xffffffffu, upto, 31);
         }
     }
 }
