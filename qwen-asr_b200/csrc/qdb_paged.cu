@@ -49,17 +49,29 @@ __device__ __forceinline__ void load8<SrcF32>(const void *p, size_t i, float *v)
 
 // Bound by memory: every row is read once and written once. Eight lanes per
 // head vector: lane i holds dims 8 i .. 8 i + 7 of both halves, the pairs that
-// rotate together, so all loads and stores are 16 bytes. A CTA has 32 vectors
+// rotate together, so all loads and stores are 16 bytes. A CTA has 16 vectors
 // of one or several rows; a row's sequence, position and page are looked up
 // once per vector by its own lanes (they hit L1).
-constexpr int AP_THREADS = 256, AP_VECS = AP_THREADS / 8;
+constexpr int AP_THREADS = 128, AP_VECS = AP_THREADS / 8;
+template <typename S>
+constexpr int ap_ctas = 16;  // per SM: enough reads in flight
+template <>
+constexpr int ap_ctas<SrcF32> = 12;  // (twice the bytes per thread, and more registers)
 
 template <typename S, typename T>
-__global__ void __launch_bounds__(AP_THREADS) append_kernel(const QdbAppendArgs a, int slots) {
+__global__ void __launch_bounds__(AP_THREADS, ap_ctas<S>) append_kernel(const QdbAppendArgs a, int slots) {
     pdl_enter();
     const int i8 = (threadIdx.x & 7) * 8, Hq = a.heads, Hkv = a.kv.kv_heads;
-    const long long vec = (long long)blockIdx.x * AP_VECS + threadIdx.x / 8;
-    const int row = (int)(vec / slots), slot = (int)(vec - (long long)row * slots);
+    int row, slot;
+    if (gridDim.x < 0xffffffffu / AP_VECS) {  // (a 64-bit division costs as much as the rest)
+        const unsigned vec = blockIdx.x * AP_VECS + threadIdx.x / 8;
+        row = vec / (unsigned)slots;
+        slot = vec - (unsigned)row * slots;
+    } else {
+        const long long vec = (long long)blockIdx.x * AP_VECS + threadIdx.x / 8;
+        row = (int)(vec / slots);
+        slot = (int)(vec - (long long)row * slots);
+    }
     const bool here = row < a.bt.rows;
     // the source does not depend on the look-ups: its loads go first
     float x[8], y[8];
