@@ -96,6 +96,23 @@ void qdb_session_free(qdb_session *s);
 int qdb_session_capacity(const qdb_session *s);
 int qdb_session_reserve(qdb_session *s, int positions);
 
+/* ---- Page pool: one K/V storage (fp16, page_size positions of every layer per
+ * page; 16, 32, 64, 128 or 256) shared by many sessions of a model. No
+ * counterpart in the reference. A session takes pages as it grows - nothing is
+ * copied - and gives them back when it is freed; a call that needs more than
+ * are left fails with "page pool exhausted" and changes nothing. Paged sessions
+ * run in qdb_prefill*, qdb_forward, qdb_forward_batch, qdb_decode_greedy(_batch)
+ * and qdb_decode_sample_batch, not in qdb_trace_step, qdb_trace_batch_step and
+ * qdb_forward_noalloc; the sessions of one call share one pool. qdb_forward and
+ * qdb_decode_greedy run them as a batch of one (hidden_out then carries 16
+ * mantissa bits). Freeing a pool detaches its sessions: their calls fail, and
+ * they are still to be freed. */
+typedef struct qdb_pool qdb_pool;
+qdb_pool *qdb_pool_create(qdb_model *m, int n_pages, int page_size);
+void qdb_pool_free(qdb_pool *p);
+int qdb_pool_free_pages(const qdb_pool *p);
+qdb_session *qdb_session_create_paged(qdb_pool *p, int initial_positions);
+
 /* ---- Prefill, replaces qwen_decoder_prefill (qwen_asr_decoder.c:262-359) ----
  * Appends seq_len positions starting at absolute position start_pos (the
  * caller's kv_cache_len, which stays authoritative on the host: the caller may
@@ -471,6 +488,13 @@ typedef struct {
  * drawn; a row with nothing else gives -1. */
 int qdb_sample(const void *logits, int type, long long row_stride, int rows, int vocab, const qdb_sampling *s,
                int *tokens_out, void *stream);
+
+/* qdb_decode_greedy_batch with every token drawn as qdb_sample draws it (the
+ * EOS mask applies). Here the arrays of `sampling` are HOST memory: parameters
+ * [n], uniform [n_steps, n]. A row without a token to draw gets -1 and goes on
+ * from token 0. Vocabularies of up to QDB_SAMPLE_MAX_VOCAB. */
+int qdb_decode_sample_batch(qdb_session *const *sessions, int n, const int *first_tokens, const int *pos,
+                            int n_steps, const qdb_sampling *sampling, int *tokens_out);
 
 /* Waits for all queued work of the model's stream. */
 int qdb_model_sync(qdb_model *m);

@@ -78,6 +78,12 @@ ABI = {
     "qdb_forward_batch": (ctypes.c_int, [ctypes.POINTER(ctypes.c_void_p), ctypes.c_int, _f32p, _i32p, _i32p, _f32p]),
     "qdb_decode_greedy_batch": (ctypes.c_int, [ctypes.POINTER(ctypes.c_void_p), ctypes.c_int, _i32p, _i32p,
                                                ctypes.c_int, _i32p]),
+    "qdb_decode_sample_batch": (ctypes.c_int, [ctypes.POINTER(ctypes.c_void_p), ctypes.c_int, _i32p, _i32p,
+                                               ctypes.c_int, ctypes.POINTER(QdbSampling), _i32p]),
+    "qdb_pool_create": (ctypes.c_void_p, [ctypes.c_void_p, ctypes.c_int, ctypes.c_int]),
+    "qdb_pool_free": (None, [ctypes.c_void_p]),
+    "qdb_pool_free_pages": (ctypes.c_int, [ctypes.c_void_p]),
+    "qdb_session_create_paged": (ctypes.c_void_p, [ctypes.c_void_p, ctypes.c_int]),
     "qdb_model_sync": (ctypes.c_int, [ctypes.c_void_p]),
     "qdb_mel_frames": (ctypes.c_int, [ctypes.c_int]),
     "qdb_build_prompt_device": (ctypes.c_int, [ctypes.c_void_p, _i32p, ctypes.c_int, ctypes.c_void_p,
@@ -235,14 +241,46 @@ class Model:
             pass
 
 
-class Session:
-    """One utterance's device KV cache (qwen_ctx_t KV fields)."""
+class PagePool:
+    """K/V pages of one model shared by many sessions (qdb_pool_*): n_pages pages
+    of page_size positions (16, 32, 64, 128 or 256)."""
 
-    def __init__(self, model: Model, capacity: int = 1024):
+    def __init__(self, model: Model, n_pages: int, page_size: int = 32):
         self.model = model
-        self.h = lib.qdb_session_create(model.h, capacity)
+        self.h = lib.qdb_pool_create(model.h, n_pages, page_size)
         if not self.h:
-            raise _err("qdb_session_create")
+            raise _err("qdb_pool_create")
+
+    @property
+    def free_pages(self) -> int:
+        return lib.qdb_pool_free_pages(self.h)
+
+    def session(self, positions: int = 0) -> "Session":
+        """A session whose cache lives in this pool's pages (positions reserved at once)."""
+        return Session(self.model, positions, pool=self)
+
+    def close(self):
+        if self.h and not _exiting[0]:
+            lib.qdb_pool_free(self.h)
+        self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class Session:
+    """One utterance's device KV cache (qwen_ctx_t KV fields), of its own or in a
+    pool's pages."""
+
+    def __init__(self, model: Model, capacity: int = 1024, pool: PagePool | None = None):
+        self.model = model
+        self.pool = pool  # (kept alive)
+        self.h = lib.qdb_session_create_paged(pool.h, capacity) if pool else lib.qdb_session_create(model.h, capacity)
+        if not self.h:
+            raise _err("qdb_session_create_paged" if pool else "qdb_session_create")
 
     @property
     def capacity(self) -> int:
@@ -683,6 +721,24 @@ def decode_greedy_batch(sessions, first_tokens, pos, n_steps: int) -> np.ndarray
                                    _ptr(out, _i32p)):
         raise _err("qdb_decode_greedy_batch")
     return out[:n_steps]
+
+
+def decode_sample_batch(sessions, first_tokens, pos, uniform, temperature=None, top_k=None, top_p=None,
+                        min_p=None) -> np.ndarray:
+    """decode_greedy_batch with drawn tokens: uniform [n_steps, n] random numbers in
+    [0, 1), parameters [n] (None = off). Returns the tokens [n_steps, n]."""
+    n = len(sessions)
+    u = np.ascontiguousarray(uniform, dtype=np.float32).reshape(-1, n)
+    f = np.ascontiguousarray(first_tokens, dtype=np.int32)
+    p = np.ascontiguousarray(pos, dtype=np.int32)
+    par = [None if v is None else np.ascontiguousarray(np.broadcast_to(np.asarray(v, t), (n,)))
+           for v, t in ((temperature, np.float32), (top_k, np.int32), (top_p, np.float32), (min_p, np.float32))]
+    s = QdbSampling(*[None if v is None else v.ctypes.data for v in par], u.ctypes.data)
+    out = np.empty((max(len(u), 1), n), np.int32)
+    if lib.qdb_decode_sample_batch(_handles(sessions), n, _ptr(f, _i32p), _ptr(p, _i32p), len(u), s,
+                                   _ptr(out, _i32p)):
+        raise _err("qdb_decode_sample_batch")
+    return out[:len(u)]
 
 
 class Decoder:

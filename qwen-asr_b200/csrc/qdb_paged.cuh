@@ -211,7 +211,13 @@ struct QdbPagedAttnArgs {
     float scale;
     uint16_t *out;
     long long out_stride;
+    uint16_t *lo;  // nullable: `out` receives the result as bf16 and lo its rest (hi + lo), whatever the cache's type
 };
+// One value of the bf16 pair: its hi part, or what that leaves.
+__device__ __forceinline__ float pair_part(float v, bool lo) {
+    const float hi = __uint_as_float((uint32_t)f32_to_bf16_rn(v) << 16);
+    return lo ? v - hi : v;
+}
 // Scratch of one call at a time: partial results [2 * ctas][16][128] with their
 // (m, l), and [ctas] counters, zero between calls.
 struct QdbDecodeScratch {

@@ -137,10 +137,18 @@ __device__ __forceinline__ Joined join(int n, int lane, ML ml, Row row) {
 }
 
 template <typename T>
-__device__ __forceinline__ void store_row4(uint16_t *dst, const Joined &j) {
+__device__ __forceinline__ void store_row4(const QdbPagedAttnArgs &a, size_t at, const Joined &j) {
     const float inv = j.l > 0.f ? 1.0f / j.l : (isnan(j.l) ? j.l : 0.f);
-    *reinterpret_cast<uint2 *>(dst) =
-        make_uint2(T::plain(j.o[0] * inv, j.o[1] * inv), T::plain(j.o[2] * inv, j.o[3] * inv));
+    float v[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) v[e] = j.o[e] * inv;
+    if (!a.lo) {
+        *reinterpret_cast<uint2 *>(a.out + at) = make_uint2(T::plain(v[0], v[1]), T::plain(v[2], v[3]));
+        return;
+    }
+    for (int p = 0; p < 2; p++)
+        *reinterpret_cast<uint2 *>((p ? a.lo : a.out) + at) =
+            make_uint2(QdbBf16::plain(pair_part(v[0], p), pair_part(v[1], p)), QdbBf16::plain(pair_part(v[2], p), pair_part(v[3], p)));
 }
 
 template <typename T, int NT>
@@ -175,8 +183,10 @@ __global__ void __launch_bounds__(DW * 32, 1)
         if (b == b0) sm.find.len0[t] = len;
         mine += (len + TILE - 1) / TILE;
         if (len == 0 && b % gridDim.x == blockIdx.x)  // the row of an empty sequence is zero
-            for (int i = 0; i < a.heads * QDB_HD / 8; i++)
+            for (int i = 0; i < a.heads * QDB_HD / 8; i++) {
                 *reinterpret_cast<uint4 *>(a.out + (size_t)b * a.out_stride + i * 8) = make_uint4(0u, 0u, 0u, 0u);
+                if (a.lo) *reinterpret_cast<uint4 *>(a.lo + (size_t)b * a.out_stride + i * 8) = make_uint4(0u, 0u, 0u, 0u);
+            }
     }
     int upto = mine;
 #pragma unroll
@@ -417,7 +427,15 @@ __global__ void __launch_bounds__(DW * 32, 1)
                     for (int d = 4; d < 32; d <<= 1) l[j][e] += __shfl_xor_sync(0xffffffffu, l[j][e], d);
             const bool begins = pair_lo >= x0;
             if (begins && ends) {  // the whole pair: its output rows
-                uint16_t *dst = a.out + (size_t)cc.b * a.out_stride + (size_t)cc.g * G * QDB_HD;
+                const size_t at = (size_t)cc.b * a.out_stride + (size_t)cc.g * G * QDB_HD;
+                auto put = [&](size_t i, float v) {
+                    if (!a.lo) {
+                        a.out[at + i] = T::plain1(v);
+                    } else {
+                        a.out[at + i] = QdbBf16::plain1(v);
+                        a.lo[at + i] = QdbBf16::plain1(pair_part(v, true));
+                    }
+                };
 #pragma unroll
                 for (int j = 0; j < NT; j++)
 #pragma unroll
@@ -427,8 +445,8 @@ __global__ void __launch_bounds__(DW * 32, 1)
                         const float inv = l[j][e] > 0.f ? 1.0f / l[j][e] : (isnan(l[j][e]) ? l[j][e] : 0.f);
 #pragma unroll
                         for (int mt = 0; mt < 8; mt++) {
-                            dst[h * QDB_HD + mt * 16 + qr] = T::plain1(o[mt][j][e] * inv);
-                            dst[h * QDB_HD + mt * 16 + 8 + qr] = T::plain1(o[mt][j][e + 2] * inv);
+                            put(h * QDB_HD + mt * 16 + qr, o[mt][j][e] * inv);
+                            put(h * QDB_HD + mt * 16 + 8 + qr, o[mt][j][e + 2] * inv);
                         }
                     }
             } else {
@@ -472,7 +490,7 @@ __global__ void __launch_bounds__(DW * 32, 1)
     }
     __syncthreads();
     auto out_row = [&](const Group &gr, int h) {
-        return a.out + (size_t)gr.b * a.out_stride + ((size_t)gr.g * G + h) * QDB_HD + lane * 4;
+        return (size_t)gr.b * a.out_stride + ((size_t)gr.g * G + h) * QDB_HD + lane * 4;
     };
     const unsigned groups = __ballot_sync(0xffffffffu, lane <= DW && sm.grp[lane <= DW ? lane : 0].some);
     const bool split = __any_sync(0xffffffffu, (groups >> lane & 1) && sm.grp[lane].c0 != sm.grp[lane].c1);
@@ -491,7 +509,7 @@ __global__ void __launch_bounds__(DW * 32, 1)
                     return *reinterpret_cast<const float4 *>(src + h * QDB_HD + lane * 4);
                 });
             if (gr.c0 == gr.c1) {
-                store_row4<T>(out_row(gr, h), j);
+                store_row4<T>(a, out_row(gr, h), j);
             } else {
                 const size_t at = (size_t)(blockIdx.x * 2 + (k ? 1 : 0)) * MAX_G + h;
                 *reinterpret_cast<float4 *>(ws.part + at * QDB_HD + lane * 4) = make_float4(j.o[0], j.o[1], j.o[2], j.o[3]);
@@ -523,7 +541,7 @@ __global__ void __launch_bounds__(DW * 32, 1)
             const Joined j = join(
                 gr.c1 - gr.c0 + 1, lane, [&](int i) { return __ldcg(ws.ml + at(i)); },
                 [&](int i) { return __ldcg(reinterpret_cast<const float4 *>(ws.part + at(i) * QDB_HD + lane * 4)); });
-            store_row4<T>(out_row(gr, h), j);
+            store_row4<T>(a, out_row(gr, h), j);
         }
     }
 }

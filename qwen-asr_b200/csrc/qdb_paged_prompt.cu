@@ -406,45 +406,50 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
             unsigned char *stage = sm.q[x] + (warp & 3) * 32 * 256;
             const unsigned inv_g = (65536u + G - 1) / G;  // r / G = r * inv_g >> 16 for r < 128
             const float scale_o = l > 0.f || isnan(l) ? inv : 0.f;
+            for (int part = 0; part < (a.lo ? 2 : 1); part++) {  // (hi, then lo of a bf16 pair)
+                auto word = [&](uint32_t x, uint32_t y) {
+                    const float u = __uint_as_float(x), v = __uint_as_float(y);
+                    return a.lo ? QdbBf16::plain(pair_part(u, part), pair_part(v, part)) : T::plain(u, v);
+                };
 #pragma unroll 1
-            for (int k = 0; k < 128; k += 64) {
-                uint32_t o[64];
-                if (nt > 0) {
-                    tm_ld64(to + k, o);
-                } else {
+                for (int k = 0; k < 128; k += 64) {
+                    uint32_t o[64];
+                    if (nt > 0) {
+                        tm_ld64(to + k, o);
+                    } else {
 #pragma unroll
-                    for (int e = 0; e < 64; e++) o[e] = 0u;
-                }
-#pragma unroll
-                for (int e = 0; e < 64; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * scale_o);
-                if (fix && real)  // non-finite values were left out of the products: add those this row sees
-                    for (int key = special * PT_N; key <= pos; key++) {
-                        const int page = paged_page(a.kv, a.bt, blk.b, key >> a.kv.page_shift);
-                        if (page < 0) continue;
-                        const uint16_t *v = a.kv.v + page * a.kv.page_stride + g * a.kv.head_stride +
-                                            (key & ((1 << a.kv.page_shift) - 1)) * a.kv.pos_stride + k;
-#pragma unroll
-                        for (int e = 0; e < 64; e++) {
-                            const float y = T::lo(v[e]);
-                            if (!isfinite(y)) o[e] = __float_as_uint(__uint_as_float(o[e]) + y);
-                        }
+                        for (int e = 0; e < 64; e++) o[e] = 0u;
                     }
 #pragma unroll
-                for (int e = 0; e < 64; e += 8)
-                    *reinterpret_cast<uint4 *>(stage + lane * 256 + ((((k + e) / 8) ^ (lane & 7)) << 4)) =
-                        make_uint4(T::plain(__uint_as_float(o[e]), __uint_as_float(o[e + 1])),
-                                   T::plain(__uint_as_float(o[e + 2]), __uint_as_float(o[e + 3])),
-                                   T::plain(__uint_as_float(o[e + 4]), __uint_as_float(o[e + 5])),
-                                   T::plain(__uint_as_float(o[e + 6]), __uint_as_float(o[e + 7])));
-            }
-            __syncwarp();
+                    for (int e = 0; e < 64; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * scale_o);
+                    if (fix && real)  // non-finite values were left out of the products: add those this row sees
+                        for (int key = special * PT_N; key <= pos; key++) {
+                            const int page = paged_page(a.kv, a.bt, blk.b, key >> a.kv.page_shift);
+                            if (page < 0) continue;
+                            const uint16_t *v = a.kv.v + page * a.kv.page_stride + g * a.kv.head_stride +
+                                                (key & ((1 << a.kv.page_shift) - 1)) * a.kv.pos_stride + k;
+#pragma unroll
+                            for (int e = 0; e < 64; e++) {
+                                const float y = T::lo(v[e]);
+                                if (!isfinite(y)) o[e] = __float_as_uint(__uint_as_float(o[e]) + y);
+                            }
+                        }
+#pragma unroll
+                    for (int e = 0; e < 64; e += 8)
+                        *reinterpret_cast<uint4 *>(stage + lane * 256 + ((((k + e) / 8) ^ (lane & 7)) << 4)) =
+                            make_uint4(word(o[e], o[e + 1]), word(o[e + 2], o[e + 3]), word(o[e + 4], o[e + 5]),
+                                       word(o[e + 6], o[e + 7]));
+                }
+                __syncwarp();
 #pragma unroll 4
-            for (int e = 0; e < 32; e += 2) {  // two rows at a time
-                const int q = e + (lane >> 4), rr = 32 * (warp & 3) + q, ii = (int)((unsigned)rr * inv_g >> 16);
-                if (ii >= nx || ii >= QP) continue;
-                uint16_t *dst = a.out + (size_t)(blk.row0 + x * QP + ii) * a.out_stride + ((size_t)g * G + rr - ii * G) * QDB_HD;
-                *reinterpret_cast<uint4 *>(dst + (lane & 15) * 8) =
-                    *reinterpret_cast<const uint4 *>(stage + q * 256 + (((lane & 15) ^ (q & 7)) << 4));
+                for (int e = 0; e < 32; e += 2) {  // two rows at a time
+                    const int q = e + (lane >> 4), rr = 32 * (warp & 3) + q, ii = (int)((unsigned)rr * inv_g >> 16);
+                    if (ii >= nx || ii >= QP) continue;
+                    uint16_t *dst = (part ? a.lo : a.out) + (size_t)(blk.row0 + x * QP + ii) * a.out_stride + ((size_t)g * G + rr - ii * G) * QDB_HD;
+                    *reinterpret_cast<uint4 *>(dst + (lane & 15) * 8) =
+                        *reinterpret_cast<const uint4 *>(stage + q * 256 + (((lane & 15) ^ (q & 7)) << 4));
+                }
+                __syncwarp();  // (the rows have been read)
             }
         }
     } else if (warp < 10) {

@@ -23,8 +23,7 @@
 
 #include "../../include/qwen_asr_b200.h"
 #include "qdb_kernels.h"
-
-#define QDB_HD 128  // head_dim (the kernels support only this)
+#include "qdb_paged.cuh"
 
 static thread_local std::string g_err;
 
@@ -100,6 +99,13 @@ struct RowScratch {
     int aseg_cap = 0;
     int *tok = nullptr;
     size_t tok_cap = 0;
+    // paged sessions: [n + 1] row starts, [n] lengths, [n][width] page tables of one call
+    int *pmeta = nullptr;
+    size_t pmeta_cap = 0;
+    QdbDecodeScratch pdec = {};  // scratch of the one-token attention over pages
+    // sampled decoding: temperature, top_p, min_p, top_k [n] each, uniform [steps][n]
+    float *samp = nullptr;
+    size_t samp_cap = 0;
 };
 
 // Scratch of the persistent batched decode step (qdb_bstep.cu), sized for its
@@ -173,12 +179,24 @@ struct qdb_model {
     int up_next = 0;
     double up_bytes = 0;
     std::vector<qdb_session *> sessions;  // live sessions (detached when the model is freed)
+    std::vector<qdb_pool *> pools;        // live page pools (emptied when the model is freed)
 };
 
 struct qdb_session {
-    qdb_model *m;  // null once the model has been freed (session detached)
+    qdb_model *m;  // null once the model (or the pool) has been freed (session detached)
     uint16_t *kc = nullptr, *vc = nullptr;
     int cap = 0;
+    qdb_pool *pool = nullptr;  // paged session: its cache is `pages` of this pool (kc, vc null)
+    std::vector<int> pages;
+};
+
+// Pages of one model's K/V cache, handed out to sessions:
+// k, v [layer][page][kv_head][slot][128] fp16.
+struct qdb_pool {
+    qdb_model *m;  // null once the model has been freed
+    uint16_t *k = nullptr, *v = nullptr;
+    int n_pages = 0, page_shift = 0;
+    std::vector<int> free;  // the next page handed out is the last one
 };
 
 extern "C" const char *qdb_last_error(void) { return g_err.c_str(); }
@@ -374,8 +392,16 @@ extern "C" void qdb_model_free(qdb_model *m) {
         s->kc = s->vc = nullptr;
         s->cap = 0;
         s->m = nullptr;
+        s->pool = nullptr;
     }
     m->sessions.clear();
+    for (qdb_pool *p : m->pools) {
+        cudaFree(p->k);
+        cudaFree(p->v);
+        p->k = p->v = nullptr;
+        p->m = nullptr;
+    }
+    m->pools.clear();
     cudaFree(m->w); cudaFree(m->norms); cudaFree(m->embed); cudaFree(m->final_norm); cudaFree(m->layers_dev);
     cudaFree(m->rope); cudaFree(m->tags); cudaFree(m->x_in);
     cudaFree(m->hidden_dev); cudaFree(m->logits_dev); cudaFree(m->done); cudaFree(m->best);
@@ -384,6 +410,7 @@ extern "C" void qdb_model_free(qdb_model *m) {
     cudaFree(r.X); cudaFree(r.XH); cudaFree(r.XL); cudaFree(r.QKV); cudaFree(r.Q); cudaFree(r.ATT); cudaFree(r.ACT);
     cudaFree(r.XH2); cudaFree(r.XL2); cudaFree(r.LOG); cudaFree(r.amax); cudaFree(r.part); cudaFree(r.acnt); cudaFree(r.rowkv); cudaFree(r.tok); cudaFree(r.err); cudaFree(r.GU); cudaFree(r.step);
     cudaFree(r.amaps); cudaFree(r.asegs);
+    cudaFree(r.pmeta); cudaFree(r.samp); cudaFree(r.pdec.part); cudaFree(r.pdec.ml); cudaFree(r.pdec.cnt);
     BatchScratch &b = m->bs;
     cudaFree(b.x); cudaFree(b.qkv); cudaFree(b.gu); cudaFree(b.part); cudaFree(b.stats); cudaFree(b.best);
     cudaFree(b.cnt); cudaFree(b.done); cudaFree(b.err); cudaFree(b.wt); cudaFree(b.prog); cudaFree(b.attn);
@@ -570,6 +597,7 @@ extern "C" void qdb_session_free(qdb_session *s) {
         cudaStreamSynchronize(m->st);
         cudaFree(s->kc);
         cudaFree(s->vc);
+        if (s->pool) s->pool->free.insert(s->pool->free.end(), s->pages.rbegin(), s->pages.rend());
         for (size_t i = 0; i < m->sessions.size(); i++)
             if (m->sessions[i] == s) {
                 m->sessions.erase(m->sessions.begin() + i);
@@ -589,6 +617,16 @@ extern "C" int qdb_session_reserve(qdb_session *s, int positions) {
     if (positions <= s->cap) return 0;
     qdb_model *m = s->m;
     if (set_dev(m)) return -1;
+    if (qdb_pool *p = s->pool) {  // more pages, nothing moves
+        const size_t need = (((size_t)positions - 1) >> p->page_shift) + 1 - s->pages.size();
+        if (need > p->free.size())
+            return fail("page pool exhausted: %zu more pages needed, %zu of %d free", need, p->free.size(), p->n_pages);
+        if (ensure_rope(m, (int)((s->pages.size() + need) << p->page_shift))) return -1;
+        s->pages.insert(s->pages.end(), p->free.rbegin(), p->free.rbegin() + need);
+        p->free.resize(p->free.size() - need);
+        s->cap = (int)(s->pages.size() << p->page_shift);
+        return 0;
+    }
     int cap = s->cap ? s->cap : 256;
     while (cap < positions) cap *= 2;
     const size_t blocks = (size_t)m->cfg.layers * m->cfg.kv_heads;
@@ -607,6 +645,68 @@ extern "C" int qdb_session_reserve(qdb_session *s, int positions) {
     s->vc = vc;
     s->cap = cap;
     return ensure_rope(m, cap);
+}
+
+// ------------------------------------------------------------------ page pools
+extern "C" qdb_pool *qdb_pool_create(qdb_model *m, int n_pages, int page_size) {
+    g_err.clear();
+    if (!m || !m->finalized) { fail("model missing or not finalized"); return nullptr; }
+    int shift = 4;
+    while (shift < 8 && (1 << shift) != page_size) shift++;
+    if ((1 << shift) != page_size) { fail("page size %d is not 16, 32, 64, 128 or 256", page_size); return nullptr; }
+    // (positions are ints)
+    if (n_pages <= 0 || n_pages > (0x7fffffff >> shift)) { fail("a pool of %d pages", n_pages); return nullptr; }
+    if (set_dev(m)) return nullptr;
+    qdb_pool *p = new qdb_pool();
+    p->m = m;
+    p->n_pages = n_pages;
+    p->page_shift = shift;
+    const size_t elems = (size_t)m->cfg.layers * n_pages * m->cfg.kv_heads * page_size * QDB_HD;
+    if (dev_alloc(&p->k, elems) || dev_alloc(&p->v, elems)) {
+        cudaFree(p->k);
+        delete p;
+        return nullptr;
+    }
+    for (int i = n_pages - 1; i >= 0; i--) p->free.push_back(i);
+    m->pools.push_back(p);
+    return p;
+}
+
+extern "C" void qdb_pool_free(qdb_pool *p) {
+    if (!p) return;
+    if (qdb_model *m = p->m) {
+        cudaSetDevice(m->device);
+        cudaStreamSynchronize(m->st);
+        // its sessions are detached like those of a freed model
+        auto &ss = m->sessions;
+        for (qdb_session *s : ss)
+            if (s->pool == p) {
+                s->m = nullptr;
+                s->pool = nullptr;
+                s->cap = 0;
+            }
+        ss.erase(std::remove_if(ss.begin(), ss.end(), [](qdb_session *s) { return !s->m; }), ss.end());
+        m->pools.erase(std::find(m->pools.begin(), m->pools.end(), p));
+        cudaFree(p->k);
+        cudaFree(p->v);
+    }
+    delete p;
+}
+
+extern "C" int qdb_pool_free_pages(const qdb_pool *p) { return p && p->m ? (int)p->free.size() : 0; }
+
+extern "C" qdb_session *qdb_session_create_paged(qdb_pool *p, int initial_positions) {
+    g_err.clear();
+    if (!p || !p->m) { fail("pool missing, or its model has been freed"); return nullptr; }
+    qdb_session *s = new qdb_session();
+    s->m = p->m;
+    s->pool = p;
+    if (initial_positions > 0 && qdb_session_reserve(s, initial_positions)) {
+        delete s;
+        return nullptr;
+    }
+    p->m->sessions.push_back(s);
+    return s;
 }
 
 // ------------------------------------------------------------------ single-utterance step
@@ -691,12 +791,34 @@ static int prep_pos(qdb_session *s, int last_pos) {
     return ensure_rope(s->m, last_pos + 1);
 }
 
+// A paged session runs as a batch of one. Its final-normed hidden state is what
+// the lm_head read: the bf16 hi + lo pair.
+static int forward_paged(qdb_session *s, const float *embed, int pos, float *hidden_out, float *logits_out) {
+    int tok = -1;
+    if (qdb_forward_batch(&s, 1, embed, &pos, &tok, logits_out)) return -1;
+    if (hidden_out) {
+        const int h = s->m->cfg.hidden;
+        std::vector<uint16_t> hi(h), lo(h);
+        CK(cudaMemcpy(hi.data(), s->m->rs.XH, 2 * (size_t)h, cudaMemcpyDeviceToHost));
+        CK(cudaMemcpy(lo.data(), s->m->rs.XL, 2 * (size_t)h, cudaMemcpyDeviceToHost));
+        for (int i = 0; i < h; i++) {
+            const uint32_t a = (uint32_t)hi[i] << 16, b = (uint32_t)lo[i] << 16;
+            float x, y;
+            memcpy(&x, &a, 4);
+            memcpy(&y, &b, 4);
+            hidden_out[i] = x + y;
+        }
+    }
+    return tok;
+}
+
 extern "C" int qdb_forward(qdb_session *s, const float *embed, int pos, float *hidden_out, float *logits_out) {
     g_err.clear();
     if (!s || !embed) return fail("null argument");
     if (!s->m) return fail("session's model has been freed");
     if (pos < 0) return fail("negative position");
     qdb_model *m = s->m;
+    if (s->pool) return forward_paged(s, embed, pos, hidden_out, logits_out);
     if (set_dev(m) || prep_pos(s, pos)) return -1;
     const size_t h = m->cfg.hidden;
     memcpy(m->h_stage, embed, h * 4);
@@ -731,6 +853,7 @@ extern "C" int qdb_decode_greedy(qdb_session *s, int first_token, int pos, int n
     qdb_model *m = s->m;
     if (first_token < 0 || first_token >= m->cfg.vocab) return fail("token %d out of range", first_token);
     if (pos < 0) return fail("negative position");
+    if (s->pool) return qdb_decode_greedy_batch(&s, 1, &first_token, &pos, n_steps, tokens_out);
     if (set_dev(m) || prep_pos(s, pos + n_steps - 1)) return -1;
     if (m->tok_cap < n_steps + 1) {
         cudaFree(m->tok_dev);
@@ -757,6 +880,7 @@ extern "C" int qdb_trace_step(qdb_session *s, int token, int pos, unsigned long 
     if (!s->m) return fail("session's model has been freed");
     qdb_model *m = s->m;
     if (token < 0 || token >= m->cfg.vocab || pos < 0) return fail("bad token or position");
+    if (s->pool) return fail("the traced step does not take paged sessions");
     const int ev = qdb_step_trace_events(m->cfg.layers);
     const size_t words = (size_t)m->grid * ev;
     if ((size_t)max_words < words) return fail("trace buffer needs %zu words", words);
@@ -840,12 +964,119 @@ struct PrefillPlan {
     bool per_row;
 };
 
+// Rows of paged sessions: the call's batch (lengths, page tables and, for
+// prompts, row starts in rs.pmeta) over this pool.
+struct PagedCall {
+    const qdb_pool *pool = nullptr;
+    QdbPagedBatch bt = {};
+};
+
+// Uploads the batch of a paged call: session i has lens[i] new rows up to
+// position ends[i] - 1 (one_row: row i is session i). The caller synchronises
+// before `host` goes.
+static int paged_call(qdb_model *m, qdb_session *const *ss, int n, const int *lens, const int *ends, bool one_row,
+                      int rows, const int *step, std::vector<int> &host, PagedCall *pc) {
+    RowScratch &r = m->rs;
+    size_t width = 1;  // a power of two: captured steps bake it in
+    for (int i = 0; i < n; i++)
+        while (width < ss[i]->pages.size()) width *= 2;
+    host.assign((size_t)n + 1 + n + width * n, 0);
+    for (int i = 0; i < n; i++) {
+        host[i + 1] = host[i] + (one_row ? 1 : lens[i]);
+        host[n + 1 + i] = ends[i];
+        std::copy(ss[i]->pages.begin(), ss[i]->pages.end(), host.begin() + 2 * n + 1 + width * i);
+    }
+    if (host.size() > r.pmeta_cap) {
+        CK(cudaStreamSynchronize(m->st));
+        cudaFree(r.pmeta);
+        r.pmeta = nullptr;
+        r.pmeta_cap = 0;
+        if (dev_alloc(&r.pmeta, host.size())) return -1;
+        r.pmeta_cap = host.size();
+    }
+    if (!r.pdec.part) {
+        if (injected("alloc")) return fail("injected allocation failure (QWEN_ASR_B200_FAULT)");
+        CK(qdb_decode_scratch_alloc(m->device, &r.pdec));
+    }
+    CK(cudaMemcpyAsync(r.pmeta, host.data(), sizeof(int) * host.size(), cudaMemcpyHostToDevice, m->st));
+    pc->pool = ss[0]->pool;
+    pc->bt = QdbPagedBatch{n,   rows,  one_row ? nullptr : r.pmeta, r.pmeta + n + 1, r.pmeta + 2 * n + 1, (int)width,
+                           r.err, step};
+    return 0;
+}
+
+// Room for position last[i] (-1: none) of every session of a call. Where a pool
+// runs out, the pages this call has taken go back.
+static int reserve_all(qdb_session *const *ss, int n, const std::vector<int> &last) {
+    std::vector<size_t> had(n);
+    for (int i = 0; i < n; i++) {
+        had[i] = ss[i]->pages.size();
+        if (last[i] < 0 || !prep_pos(ss[i], last[i])) continue;
+        for (int k = i; k >= 0; k--)
+            if (qdb_pool *p = ss[k]->pool) {
+                auto &pg = ss[k]->pages;
+                p->free.insert(p->free.end(), pg.rbegin(), pg.rend() - had[k]);
+                pg.resize(had[k]);
+                ss[k]->cap = (int)(had[k] << p->page_shift);
+            }
+        return -1;
+    }
+    return 0;
+}
+
+// Whether the sessions of a call are paged (1), contiguous (0), or cannot run together (-1).
+static int paged_kind(qdb_session *const *ss, int n) {
+    for (int i = 1; i < n; i++)
+        if (ss[i]->pool != ss[0]->pool)
+            return fail("session %d: sessions of one call must share one page pool, or all be without one", i);
+    return ss[0]->pool ? 1 : 0;
+}
+
+// Append and attention of one layer over pages: QKV rows in rs.QKV, the
+// O-projection's bf16 split out.
+static int paged_layer(qdb_model *m, int l, int n, const PagedCall &pc) {
+    RowScratch &r = m->rs;
+    const qdb_pool *p = pc.pool;
+    const QdbLayerW &lw = m->layers_host[l];
+    const int Hq = m->cfg.heads, Hkv = m->cfg.kv_heads;
+    const long long pos = QDB_HD, head = pos << p->page_shift, page = head * Hkv;
+    const size_t at = (size_t)l * p->n_pages * page;
+    QdbAppendArgs a{};
+    a.kv = QdbPagedKV{p->k + at, p->v + at, p->n_pages, p->page_shift, Hkv, page, head, pos};
+    a.bt = pc.bt;
+    a.qkv = r.QKV;
+    a.row_stride = m->qd + 2 * m->kvd;
+    a.heads = Hq;
+    a.q_norm = lw.q_norm;
+    a.k_norm = lw.k_norm;
+    a.eps = m->cfg.eps;
+    a.rope = m->rope;
+    a.rope_len = m->rope_cap;
+    a.q_out = reinterpret_cast<uint16_t *>(r.Q);
+    a.q_stride = m->qd;
+    CK(qdb_launch_paged_append(a, QDB_TYPE_F32, QDB_TYPE_F16, m->st));
+    QdbPagedAttnArgs t{};
+    t.kv = a.kv;
+    t.bt = pc.bt;
+    t.q = a.q_out;
+    t.q_stride = m->qd;
+    t.heads = Hq;
+    t.scale = 1.0f / sqrtf((float)QDB_HD);
+    t.out = r.XH;
+    t.lo = r.XL;
+    t.out_stride = m->qd;
+    if (pc.bt.q_starts) CK(qdb_launch_paged_prompt(t, QDB_TYPE_F16, m->st));
+    else CK(qdb_launch_paged_decode(t, QDB_TYPE_F16, r.pdec, m->st));
+    return 0;
+}
+
 // One transformer stack over the rows already in rs.X. pf: prefill rows
 // (causal attention over each session's cache, tensor cores); null: decode
 // rows, row b uses rowkv[b] at position rowkv[b].pos + pos_off (+ *step).
+// pc: rows of paged sessions (prompts or one per session) instead.
 static int run_rows(qdb_model *m, int n, const PrefillPlan *pf, const QdbRowKV *row0_dev, int pos_off, int max_ctx = 1,
-                    const int *step = nullptr) {
-    const bool single = pf != nullptr;
+                    const int *step = nullptr, const PagedCall *pc = nullptr) {
+    const bool single = pf != nullptr || pc != nullptr;  // (neither needs the contiguous decode attention's scratch)
     if (launch_gate()) return -1;
     RowScratch &r = m->rs;
     const int h = m->cfg.hidden, I = m->cfg.intermediate, Hq = m->cfg.heads, Hkv = m->cfg.kv_heads;
@@ -895,7 +1126,9 @@ static int run_rows(qdb_model *m, int n, const PrefillPlan *pf, const QdbRowKV *
         CK(qdb_launch_rmsnorm_rows(r.X, lw.in_norm, r.XH, r.XL, n, h, m->cfg.eps, m->st, qkv_split ? r.QKV : nullptr,
                                    qkvd));
         if (gemm(lw.qkv, r.QKV, qkvd, h, 0, qkv_split)) return -1;
-        if (single) {
+        if (pc) {
+            if (paged_layer(m, l, n, *pc)) return -1;
+        } else if (single) {
             if (pf->per_row)
                 CK(qdb_launch_qk_rope_append(r.QKV, r.Q, row0_dev, 0, l, n, Hq, Hkv, lw.q_norm, lw.k_norm, m->rope,
                                              m->cfg.eps, m->st));
@@ -947,7 +1180,8 @@ static int check_rows_err(qdb_model *m) {
     CK(cudaMemcpy(ev, m->rs.err, sizeof(ev), cudaMemcpyDeviceToHost));
     if (ev[0]) {
         cudaMemset(m->rs.err, 0, sizeof(ev));
-        return fail("device error code %d in a tensor-core GEMM (a bounded wait ran out)", ev[0]);
+        return fail("device error code %d in a tensor-core GEMM (%s)", ev[0],
+                    ev[0] == QDB_ERR_BOUNDS ? "an access refused by a bounds check" : "a bounded wait ran out");
     }
     return 0;
 }
@@ -975,10 +1209,26 @@ static int prefill_rows(qdb_session *const *ss, int nsess, const int *lens, cons
     if (total > (1 << 22)) return fail("prefill of %lld rows exceeds the 4M-row limit", total);
     const int T = (int)total;
     if (set_dev(m)) return -1;
+    if (paged_kind(ss, nsess) < 0) return -1;
+    std::vector<int> last(nsess, -1);
     for (int i = 0; i < nsess; i++)
-        if (lens[i] && prep_pos(ss[i], starts[i] + lens[i] - 1)) return -1;
+        if (lens[i]) last[i] = starts[i] + lens[i] - 1;
+    if (reserve_all(ss, nsess, last)) return -1;
     if (ensure_rows(m, T, false)) return -1;
     RowScratch &r = m->rs;
+    if (ss[0]->pool) {
+        std::vector<int> ends(nsess), host;
+        for (int i = 0; i < nsess; i++) ends[i] = starts[i] + lens[i];
+        PagedCall pc;
+        CK(cudaMemcpyAsync(r.X, embeds, (size_t)T * m->cfg.hidden * 4,
+                           device_ptr ? cudaMemcpyDeviceToDevice : cudaMemcpyHostToDevice, m->st));
+        const int rc = paged_call(m, ss, nsess, lens, ends.data(), false, T, nullptr, host, &pc) ||
+                       run_rows(m, T, nullptr, nullptr, 0, 1, nullptr, &pc);
+        const cudaError_t e = cudaStreamSynchronize(m->st);  // (`host` outlives the copy)
+        if (rc) return -1;
+        if (e != cudaSuccess) return fail("prefill: %s", cudaGetErrorString(e));
+        return check_rows_err(m);
+    }
     if (nsess > r.aseg_cap) {
         cudaFree(r.amaps);
         cudaFree(r.asegs);
@@ -1054,8 +1304,10 @@ extern "C" int qdb_prefill_batch_device(qdb_session *const *sessions, int n, con
     return prefill_rows(sessions, n, seq_lens, start_pos, embeds_dev, true);
 }
 
+// pc (sessions that may be paged): their batch, whose lengths count the row at
+// pos (+ *step); pool null: contiguous sessions, in rs.rowkv.
 static int batch_setup(qdb_session *const *ss, int n, const int *pos, int extra_steps, qdb_model **mo,
-                       int *max_pos = nullptr) {
+                       int *max_pos = nullptr, PagedCall *pc = nullptr, const bool with_step = false) {
     if (!ss || n <= 0 || !pos) return fail("bad batch arguments");
     qdb_model *m = ss[0] ? ss[0]->m : nullptr;
     if (!m) return fail("null session or session's model has been freed");
@@ -1063,27 +1315,39 @@ static int batch_setup(qdb_session *const *ss, int n, const int *pos, int extra_
         if (!ss[b] || ss[b]->m != m) return fail("row %d: sessions must share one model", b);
         if (pos[b] < 0) return fail("row %d: negative position", b);
     }
+    const int kind = paged_kind(ss, n);
+    if (kind < 0) return -1;
+    if (kind && !pc) return fail("this call does not take paged sessions");
     if (set_dev(m) || ensure_rows(m, n, true)) return -1;
     std::vector<QdbRowKV> rk(n);
-    for (int b = 0; b < n; b++) {
-        if (prep_pos(ss[b], pos[b] + extra_steps)) return -1;
-    }
+    std::vector<int> last(n);
+    for (int b = 0; b < n; b++) last[b] = pos[b] + extra_steps;
+    if (reserve_all(ss, n, last)) return -1;
     for (int b = 0; b < n; b++) rk[b] = QdbRowKV{ss[b]->kc, ss[b]->vc, ss[b]->cap, pos[b]};
     if (max_pos) {
         *max_pos = 0;
         for (int b = 0; b < n; b++) *max_pos = std::max(*max_pos, pos[b]);
     }
+    *mo = m;
+    if (kind) {
+        std::vector<int> ends(n), host;
+        for (int b = 0; b < n; b++) ends[b] = pos[b] + 1;
+        if (paged_call(m, ss, n, nullptr, ends.data(), true, n, with_step ? m->rs.step : nullptr, host, pc)) return -1;
+        CK(cudaStreamSynchronize(m->st));  // (`host` is a stack vector)
+        return 0;
+    }
     CK(cudaMemcpyAsync(m->rs.rowkv, rk.data(), sizeof(QdbRowKV) * n, cudaMemcpyHostToDevice, m->st));
     CK(cudaStreamSynchronize(m->st));  // rk is a stack vector
-    *mo = m;
     return 0;
 }
 
-static int batch_tail(qdb_model *m, int n, int *tok_dev, const int *step = nullptr) {
+// The rows' tokens: the greedy ones, or drawn as `sa` says.
+static int batch_tail(qdb_model *m, int n, int *tok_dev, const int *step = nullptr, const QdbSampleArgs *sa = nullptr) {
     RowScratch &r = m->rs;
     CK(qdb_launch_rmsnorm_rows(r.X, m->final_norm, r.XH, r.XL, n, m->cfg.hidden, m->cfg.eps, m->st));
     CK(qdb_launch_gemm_tc(m->embed, r.XH, r.XL, r.LOG, n, m->cfg.vocab, m->cfg.hidden, 0, 1, r.err, m->st));
-    CK(qdb_launch_argmax_rows(r.LOG, n, m->cfg.vocab, m->mask_eos, tok_dev, m->st, step, r.amax));
+    if (sa) CK(qdb_launch_sample(*sa, QDB_TYPE_F32, m->st));
+    else CK(qdb_launch_argmax_rows(r.LOG, n, m->cfg.vocab, m->mask_eos, tok_dev, m->st, step, r.amax));
     return 0;
 }
 
@@ -1298,10 +1562,11 @@ extern "C" int qdb_forward_batch(qdb_session *const *sessions, int n, const floa
     qdb_model *m = nullptr;
     if (!embeds || !tokens_out) return fail("null argument");
     int maxp = 0;
-    if (batch_setup(sessions, n, pos, 0, &m, &maxp) || ensure_tok(m, n)) return -1;
+    PagedCall pc;
+    if (batch_setup(sessions, n, pos, 0, &m, &maxp, &pc) || ensure_tok(m, n)) return -1;
     CK(cudaMemcpyAsync(m->rs.X, embeds, (size_t)n * m->cfg.hidden * 4, cudaMemcpyHostToDevice, m->st));
     RowScratch &r = m->rs;
-    if (bstep_usable(m, n)) {
+    if (!pc.pool && bstep_usable(m, n)) {
         if (ensure_bstep(m) ||
             launch_bstep(m, n, maxp + 1, nullptr, r.X, r.tok, logits_out ? r.LOG : nullptr, 0,
                          bstep_splits(m, n, maxp + 1)))
@@ -1313,7 +1578,9 @@ extern "C" int qdb_forward_batch(qdb_session *const *sessions, int n, const floa
         CK(cudaStreamSynchronize(m->st));
         return check_bstep_err(m);
     }
-    auto step = [&]() { return run_rows(m, n, nullptr, r.rowkv, 0, maxp + 1) || batch_tail(m, n, r.tok); };
+    auto step = [&]() {
+        return run_rows(m, n, nullptr, r.rowkv, 0, maxp + 1, nullptr, pc.pool ? &pc : nullptr) || batch_tail(m, n, r.tok);
+    };
     const int S = std::min(64, std::max(1, (maxp + 1 + 64 * QDB_AR_ITERS - 1) / (64 * QDB_AR_ITERS)));
     // the captured launches bake in the row count, the split count, every
     // scratch pointer, the RoPE table (reallocated when a session grows past
@@ -1321,7 +1588,9 @@ extern "C" int qdb_forward_batch(qdb_session *const *sessions, int n, const floa
     auto graph_key = [&]() {
         return std::vector<const void *>{(const void *)(intptr_t)n, (const void *)(intptr_t)S,
                                          (const void *)(intptr_t)m->mask_eos, m->rope, r.X, r.XH, r.XL, r.QKV, r.Q,
-                                         r.ATT, r.ACT, r.LOG, r.part, r.acnt, r.GU, r.tok, r.err, r.rowkv, r.amax};
+                                         r.ATT, r.ACT, r.LOG, r.part, r.acnt, r.GU, r.tok, r.err, r.rowkv, r.amax,
+                                         pc.pool, pc.pool ? pc.pool->k : nullptr, r.pmeta,
+                                         (const void *)(intptr_t)pc.bt.table_stride, r.pdec.part};
     };
     const std::vector<const void *> key = graph_key();
     if (m->fb_exec && key == m->fb_key) {
@@ -1383,18 +1652,21 @@ extern "C" int qdb_trace_batch_step(qdb_session *const *sessions, int n, const f
     return check_bstep_err(m) ? -1 : ev;
 }
 
-extern "C" int qdb_decode_greedy_batch(qdb_session *const *sessions, int n, const int *first_tokens, const int *pos,
-                                       int n_steps, int *tokens_out) {
+// The batched device-resident loop: greedy, or (sampling given, host arrays)
+// with drawn tokens.
+static int decode_loop(qdb_session *const *sessions, int n, const int *first_tokens, const int *pos, int n_steps,
+                       const qdb_sampling *sampling, int *tokens_out) {
     g_err.clear();
     qdb_model *m = nullptr;
     if (!first_tokens || (n_steps > 0 && !tokens_out)) return fail("null argument");
     if (n_steps <= 0) return 0;
     int maxp = 0;
-    if (batch_setup(sessions, n, pos, n_steps - 1, &m, &maxp) || ensure_tok(m, (size_t)n * (n_steps + 1))) return -1;
+    PagedCall pc;
+    if (batch_setup(sessions, n, pos, n_steps - 1, &m, &maxp, &pc, true) || ensure_tok(m, (size_t)n * (n_steps + 1))) return -1;
     for (int b = 0; b < n; b++)
         if (first_tokens[b] < 0 || first_tokens[b] >= m->cfg.vocab) return fail("row %d: token out of range", b);
     CK(cudaMemcpyAsync(m->rs.tok, first_tokens, sizeof(int) * n, cudaMemcpyHostToDevice, m->st));
-    if (bstep_usable(m, n)) {
+    if (!pc.pool && !sampling && bstep_usable(m, n)) {
         if (ensure_bstep(m)) return -1;
         const int S = bstep_splits(m, n, maxp + n_steps);
         for (int i = 0; i < n_steps; i++)
@@ -1412,9 +1684,31 @@ extern "C" int qdb_decode_greedy_batch(qdb_session *const *sessions, int n, cons
     RowScratch &r = m->rs;
     const int ctx_last = maxp + n_steps;
     CK(cudaMemsetAsync(r.step, 0, sizeof(int), m->st));
+    QdbSampleArgs sa{};
+    if (sampling) {
+        const size_t total = (size_t)n * (4 + n_steps);
+        if (total > r.samp_cap) {
+            CK(cudaStreamSynchronize(m->st));
+            cudaFree(r.samp);
+            r.samp = nullptr;
+            r.samp_cap = 0;
+            if (dev_alloc(&r.samp, total)) return -1;
+            r.samp_cap = total;
+        }
+        const void *src[5] = {sampling->temperature, sampling->top_p, sampling->min_p, sampling->top_k, sampling->uniform};
+        for (int i = 0; i < 5; i++)
+            if (src[i])
+                CK(cudaMemcpyAsync(r.samp + (size_t)i * n, src[i], sizeof(float) * n * (i < 4 ? 1 : n_steps),
+                                   cudaMemcpyHostToDevice, m->st));
+        sa = QdbSampleArgs{r.LOG, m->cfg.vocab, n, m->cfg.vocab, src[0] ? r.samp : nullptr,
+                           src[3] ? reinterpret_cast<int *>(r.samp + 3 * (size_t)n) : nullptr,
+                           src[1] ? r.samp + n : nullptr, src[2] ? r.samp + 2 * (size_t)n : nullptr,
+                           r.samp + 4 * (size_t)n, m->mask_eos, r.tok + n, r.step};
+    }
     auto one_step = [&]() -> int {
         CK(qdb_launch_embed_rows(m->embed, r.tok, r.X, n, m->cfg.hidden, m->cfg.vocab, m->st, r.step));
-        if (run_rows(m, n, nullptr, r.rowkv, 0, ctx_last, r.step) || batch_tail(m, n, r.tok + n, r.step))
+        if (run_rows(m, n, nullptr, r.rowkv, 0, ctx_last, r.step, pc.pool ? &pc : nullptr) ||
+            batch_tail(m, n, r.tok + n, r.step, sampling ? &sa : nullptr))
             return -1;
         CK(qdb_launch_step_advance(r.step, m->st));
         return 0;
@@ -1442,6 +1736,20 @@ extern "C" int qdb_decode_greedy_batch(qdb_session *const *sessions, int n, cons
     return check_rows_err(m);
 }
 
+extern "C" int qdb_decode_greedy_batch(qdb_session *const *sessions, int n, const int *first_tokens, const int *pos,
+                                       int n_steps, int *tokens_out) {
+    return decode_loop(sessions, n, first_tokens, pos, n_steps, nullptr, tokens_out);
+}
+
+extern "C" int qdb_decode_sample_batch(qdb_session *const *sessions, int n, const int *first_tokens, const int *pos,
+                                       int n_steps, const qdb_sampling *sampling, int *tokens_out) {
+    g_err.clear();
+    if (!sampling || (n_steps > 0 && !sampling->uniform)) return fail("sampled decoding needs random numbers");
+    if (sessions && n > 0 && sessions[0] && sessions[0]->m && sessions[0]->m->cfg.vocab > QDB_SAMPLE_MAX_VOCAB)
+        return fail("sampling serves vocabularies of up to %d", QDB_SAMPLE_MAX_VOCAB);
+    return decode_loop(sessions, n, first_tokens, pos, n_steps, sampling, tokens_out);
+}
+
 // ------------------------------------------------------------------ decode step without allocation
 // Scratch of qdb_forward_noalloc: the persistent step's tagged inter-CTA
 // vectors, followed by its argmax key, completion counter and error words.
@@ -1458,6 +1766,7 @@ extern "C" int qdb_forward_noalloc(qdb_session *s, const float *embed_dev, int p
     if (!s || !embed_dev || !token_dev) return fail("null argument");
     if (!s->m) return fail("session's model has been freed");
     qdb_model *m = s->m;
+    if (s->pool) return fail("the no-allocation step does not take paged sessions");
     if (m->device < 0 || m->device >= 64) return fail("device index %d out of range", m->device);
     if (pos < 0) return fail("negative position");
     // Nothing may grow here (growing allocates): the session and the RoPE
