@@ -53,6 +53,12 @@ struct QdbHalf {
         const __half2 r = __floats2half2_rn(a, b);
         return *reinterpret_cast<const uint32_t *>(&r);
     }
+    // acc + 0 * w of both halves: NaN from the first non-finite value on
+    static __device__ __forceinline__ uint32_t zero_times(uint32_t w, uint32_t acc) {
+        const __half2 r = __hfma2(*reinterpret_cast<const __half2 *>(&w), __half2half2(__ushort_as_half(0)),
+                                  *reinterpret_cast<const __half2 *>(&acc));
+        return *reinterpret_cast<const uint32_t *>(&r);
+    }
     static __device__ __forceinline__ bool any_nonfinite(uint32_t w) {
         return (w & 0x7c00u) == 0x7c00u || (w & 0x7c000000u) == 0x7c000000u;
     }
@@ -73,6 +79,11 @@ struct QdbBf16 {
     static __device__ __forceinline__ uint16_t one(float f) { return f32_to_bf16_rn(f); }
     static __device__ __forceinline__ uint16_t plain1(float f) { return one(f); }
     static __device__ __forceinline__ uint32_t plain(float a, float b) { return pack(a, b); }
+    static __device__ __forceinline__ uint32_t zero_times(uint32_t w, uint32_t acc) {
+        const __nv_bfloat162 r = __hfma2(*reinterpret_cast<const __nv_bfloat162 *>(&w), __bfloat162bfloat162(__ushort_as_bfloat16(0)),
+                                         *reinterpret_cast<const __nv_bfloat162 *>(&acc));
+        return *reinterpret_cast<const uint32_t *>(&r);
+    }
     static __device__ __forceinline__ bool any_nonfinite(uint32_t w) {
         return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
     }

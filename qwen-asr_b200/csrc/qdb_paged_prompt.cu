@@ -1,7 +1,7 @@
 // qdb_paged_prompt.cu - causal attention of packed prompts over a paged KV
 // cache on the tensor cores (tcgen05).
 //
-// A CTA owns one key head and one block of a sequence's new rows: two tiles of
+// An item is one key head and one block of a sequence's new rows: two tiles of
 // 128 MMA rows (row r = position r / G, head r % G of the group), which share
 // every K and V tile of 128 keys. It is bound by the tensor cores and by the
 // exponentials (128 x 128 of them per tile take as long on the special
@@ -10,15 +10,17 @@
 // a row tile's next scores are there before its softmax of this tile ends.
 //   warps 0-3, 4-7  softmax of tile 0, 1: thread = row = TMEM lane
 //   warp 8          issues S = Q K^T      (two warps, since waiting for the next
-//   warp 9          issues O += P V        operands takes half as long as a product)
-//   warps 10, 11    copy Q and the pages of K (ring of 2 tiles), of V (ring of 3):
-//                   two, since a page of 16 positions takes as many instructions as
-//                   one of 128
+//   warp 9          issues O += P V        operands takes half as long as a product),
+//                   and clears what V holds behind the last visible key
+//   warp 10         announces the items, copies Q and the pages of K (ring of 2 tiles)
+//   warp 11         copies the pages of V (ring of 3)
 // TMEM: S (128 columns, read into registers at once, so one serves both row
 // tiles in turn), P0, P1 (64 columns of packed 16-bit pairs, the A operand of
 // the second product), O0, O1 (128 columns each). No product waits for another
 // one's TMEM columns but through the softmax.
 // V is used as loaded (keys along K, dims along N).
+// One CTA per SM walks through items, taking the next from the launch queue:
+// its look-ups, copies and first scores run while the last one's output leaves.
 //   m, l            running maximum and sum per row in f32; O is rescaled only
 //                   when the maximum grows by more than 2^8, so numerator and
 //                   denominator always share one m
@@ -39,17 +41,33 @@ constexpr int PT_N = 128;                 // keys per tile
 constexpr int PT_KS = 2, PT_VS = 3;       // K and V tiles in shared memory
 constexpr uint32_t PT_HALF = 128 * 128;   // bytes of [128 rows][64 dims]
 constexpr uint32_t PT_TILE = 2 * PT_HALF;
-constexpr int PT_PART = 3;                // tiles that some row sees only in part: 256 positions touch 3
+constexpr int PT_PART = 4;                // its barriers: more than such tiles in the ring
+constexpr int PT_ITEMS = 4;               // announced items
 constexpr float PT_RAISE = 8.0f;          // log2 growth of the maximum that is let pass
+
+// One item's rows.
+struct Block {
+    int b, row0, n, pos0;  // sequence, its first row here, rows (positions) here, position of the first
+    bool any;
+};
+struct Item {
+    Block blk;
+    int g;          // key head
+    int nonfinite;  // set where values had to be cleared
+};
 
 struct PromptSmem {
     unsigned char q[2][PT_TILE];
     unsigned char k[PT_KS][PT_TILE], v[PT_VS][PT_TILE];
-    unsigned long long q_full, k_full[PT_KS], k_empty[PT_KS], v_full[PT_VS], v_empty[PT_VS], s_full[2], s_read, p_full[2], o_done[2], drain[2];
-    unsigned long long v_part[PT_PART], v_clean[PT_PART];  // V of the tiles seen in part: landed, cleared
+    unsigned long long q_full, q_empty, k_full[PT_KS], k_empty[PT_KS], v_full[PT_VS], v_empty[PT_VS];
+    unsigned long long s_full[2], s_read, p_full[2], o_done[2], drain[2];
+    unsigned long long v_clean[PT_PART];  // one half of a V tile seen in part is cleared
+    unsigned long long item_full[PT_ITEMS], item_empty[PT_ITEMS];
+    Item item[PT_ITEMS];
+    alignas(16) uint64_t stolen[2];  // answer to a request for another CTA's number
+    unsigned long long stolen_bar;
     uint32_t tmem;
     int abort;
-    int nonfinite;
 };
 
 // ---- tcgen05
@@ -168,12 +186,6 @@ __device__ __forceinline__ bool wait_on(PromptSmem &sm, uint32_t bar, unsigned p
     return true;
 }
 
-// The CTA's block of rows.
-struct Block {
-    int b, row0, n, pos0;  // sequence, its first row here, rows (positions) here, position of the first
-    bool any;
-};
-
 // Blocks of bq rows: sequence b's begin at number q_starts[b] / bq + b, which
 // leaves room for every sequence's last, partly filled block (the numbers
 // behind it are empty). The blocks with the longest histories come first.
@@ -207,7 +219,26 @@ __device__ Block find_block(const QdbPagedAttnArgs &a, int bq, int i, int lane) 
     return k;
 }
 
-template <typename T>
+// What the roles derive from a block.
+struct Shape {
+    int b, row0, pos0, g;
+    int n0, n1;                    // positions of row tiles 0 and 1
+    int t0, t1, tiles, end;        // key tiles they need, and all; keys
+    int special, parts;            // first tile that some row does not see whole; number of such tiles
+    __device__ __forceinline__ Shape(const Block &k, int g, int QP) : b(k.b), row0(k.row0), pos0(k.pos0), g(g) {
+        n0 = min(k.n, QP);
+        n1 = k.n - n0;
+        const int end0 = max(pos0 + n0, 0), end1 = n1 > 0 ? max(pos0 + k.n, 0) : 0;
+        t0 = (end0 + PT_N - 1) / PT_N;
+        t1 = (end1 + PT_N - 1) / PT_N;
+        tiles = max(t0, t1);
+        end = max(end0, end1);
+        special = max(pos0 + 1, 0) / PT_N;
+        parts = max(tiles - special, 0);
+    }
+};
+
+template <typename T, bool PAIR>  // PAIR: the output as a bf16 pair (a.out, a.lo)
 __global__ void __launch_bounds__(PT_THREADS, 1)
     prompt_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
                   const __grid_constant__ CUtensorMap mv, const __grid_constant__ QdbPagedAttnArgs a) {
@@ -215,10 +246,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
     PromptSmem &sm = *reinterpret_cast<PromptSmem *>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const int Hkv = a.kv.kv_heads, G = a.heads / Hkv, QP = 128 / G;  // positions per row tile
-    const int g = blockIdx.x % Hkv;
     int *err = a.bt.err;
     if (t == 0) {
         bar_init(smem_u32(&sm.q_full), 1);
+        bar_init(smem_u32(&sm.q_empty), 1);
         for (int s = 0; s < PT_KS; s++) {
             bar_init(smem_u32(&sm.k_full[s]), 1);
             bar_init(smem_u32(&sm.k_empty[s]), 1);
@@ -231,16 +262,16 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
             bar_init(smem_u32(&sm.s_full[x]), 1);
             bar_init(smem_u32(&sm.p_full[x]), 128);
             bar_init(smem_u32(&sm.o_done[x]), 1);
+            bar_init(smem_u32(&sm.drain[x]), 1);
         }
         bar_init(smem_u32(&sm.s_read), 128);
-        for (int k = 0; k < PT_PART; k++) {
-            bar_init(smem_u32(&sm.v_part[k]), 1);
-            bar_init(smem_u32(&sm.v_clean[k]), 256);
+        for (int k = 0; k < PT_PART; k++) bar_init(smem_u32(&sm.v_clean[k]), 1);
+        for (int k = 0; k < PT_ITEMS; k++) {
+            bar_init(smem_u32(&sm.item_full[k]), 1);
+            bar_init(smem_u32(&sm.item_empty[k]), 11);  // every warp but the announcing one
         }
-        bar_init(smem_u32(&sm.drain[0]), 1);
-        bar_init(smem_u32(&sm.drain[1]), 1);
+        bar_init(smem_u32(&sm.stolen_bar), 1);
         sm.abort = 0;
-        sm.nonfinite = 0;
         fence_bar_init();
         asm volatile("prefetch.tensormap [%0];" ::"l"(&mq) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&mk) : "memory");
@@ -248,14 +279,6 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
     }
     __syncthreads();
     pdl_enter();
-    const Block blk = find_block(a, 2 * QP, blockIdx.x / Hkv, lane);
-    if (!blk.any) return;
-    // tile x: rows of positions [x * QP, x * QP + nx); keys it needs, in tiles
-    const int n0 = min(blk.n, QP), n1 = blk.n - n0;
-    const int end0 = max(blk.pos0 + n0, 0), end1 = n1 > 0 ? max(blk.pos0 + blk.n, 0) : 0;
-    const int t0 = (end0 + PT_N - 1) / PT_N, t1 = (end1 + PT_N - 1) / PT_N, tiles = max(t0, t1), end = max(end0, end1);
-    // tiles from here on are not seen whole by every row
-    const int special = max(blk.pos0 + 1, 0) / PT_N;
     // (after the wait for the kernel before: a CTA of it that shares the SM must
     // never find the columns taken by one that waits for it)
     if (warp == 8) {
@@ -271,314 +294,416 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
     // registers as launched (168 x 384) shared out anew: 208 x 256 + 88 x 128
     if (warp < 8) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     else asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    // Every role walks through the CTA's items on its own, as warp 10 announces
+    // them, and keeps its own counts of the barriers' phases.
+    bool ok = true;
+    auto wait = [&](uint32_t bar, unsigned parity) { return __all_sync(0xffffffffu, wait_on(sm, bar, parity, err)); };
+    int item = 0;
+    Block blk;
+    int g = 0;
+    auto next_item = [&]() -> bool {  // the announced block; false: no more (or given up)
+        const int k = item % PT_ITEMS;
+        ok = wait(smem_u32(&sm.item_full[k]), (item / PT_ITEMS) & 1);
+        if (!ok) return false;
+        blk = sm.item[k].blk;
+        g = sm.item[k].g;
+        item++;
+        return blk.any;
+    };
+    auto item_done = [&] {  // this warp no longer needs the announcement
+        __syncwarp();
+        if (lane == 0) bar_arrive(smem_u32(&sm.item_empty[(item - 1) % PT_ITEMS]));
+    };
+
+    // Half the dims of a V tile that some row sees only in part: behind the last
+    // visible key they are zero, non-finite values are zero and noted.
+    auto clear_v = [&](unsigned st, int half, int keys) {
+        uint4 *v = reinterpret_cast<uint4 *>(sm.v[st] + half * PT_HALF);
+        const int mine = keys * 8;  // 16 bytes of key e / 8 (the swizzle moves them within their row only)
+        for (int e = mine + lane; e < (int)(PT_HALF / 16); e += 32) v[e] = make_uint4(0u, 0u, 0u, 0u);
+        uint32_t acc = 0;
+#pragma unroll 8
+        for (int e = lane; e < mine; e += 32) {
+            const uint4 w = v[e];
+            acc |= T::zero_times(w.w, T::zero_times(w.z, T::zero_times(w.y, T::zero_times(w.x, 0))));
+        }
+        if (T::any_nonfinite(acc)) {
+            *reinterpret_cast<volatile int *>(&sm.item[(item - 1) % PT_ITEMS].nonfinite) = 1;
+            __threadfence_block();
+            for (int e = lane; e < mine; e += 32) {
+                const uint4 w = v[e];
+                v[e] = make_uint4(T::clear_nonfinite(w.x), T::clear_nonfinite(w.y), T::clear_nonfinite(w.z),
+                                  T::clear_nonfinite(w.w));
+            }
+        }
+        fence_async();  // (before the product's reads, and the next copy into the stage)
+        __syncwarp();
+    };
+
     if (warp < 8) {
         // ------------------------------------------------ softmax of row tile x
-        const int x = warp >> 2, r = t & 127, nx = x ? n1 : n0, nt = x ? t1 : t0;
-        const int i = r / G;  // position in the tile
-        const int pos = blk.pos0 + x * QP + i;
-        const bool real = i < nx && i < QP;
-        const int whole = max(blk.pos0 + x * QP + 1, 0) / PT_N;  // tiles before this one need no mask
+        const int x = warp >> 2, r = t & 127;
+        const int i = r / G;  // position in the row tile
         const uint32_t ts = tm + ((uint32_t)(32 * (warp & 3)) << 16), tp = ts + 128 + x * 64, to = ts + 256 + x * 128;
         const float c = a.scale * 1.4426950408889634f;
         constexpr float shift = T::code == QDB_TYPE_F16 ? 6.f : 0.f;  // keeps f16 weights down to 2^-30 of the largest
-        float m = -INFINITY, l = 0.f;
-        bool ok = true;
-        // Half x of V's dims of a tile that some row sees only in part.
-        auto clear_v = [&](int j) {
-            if (!wait_on(sm, smem_u32(&sm.v_part[j - special]), 0, err)) return false;
-            uint4 *v = reinterpret_cast<uint4 *>(sm.v[j % PT_VS] + x * PT_HALF);
-            bool odd = false, wrote = false;
-#pragma unroll
-            for (int e = r; e < (int)(PT_HALF / 16); e += 128) {
-                // 16 bytes of key e / 8 (the swizzle moves them within their row only)
-                uint4 w = v[e];
-                if (j * PT_N + (e >> 3) >= end) {
-                    v[e] = make_uint4(0u, 0u, 0u, 0u);
-                    wrote = true;
-                } else if (T::any_nonfinite(w.x) | T::any_nonfinite(w.y) | T::any_nonfinite(w.z) | T::any_nonfinite(w.w)) {
-                    v[e] = make_uint4(T::clear_nonfinite(w.x), T::clear_nonfinite(w.y), T::clear_nonfinite(w.z),
-                                      T::clear_nonfinite(w.w));
-                    odd = wrote = true;
-                }
-            }
-            if (odd) {
-                *reinterpret_cast<volatile int *>(&sm.nonfinite) = 1;
-                __threadfence_block();
-            }
-            if (wrote) fence_async();
-            bar_arrive(smem_u32(&sm.v_clean[j - special]));
-            return true;
-        };
-        // The output product of tile j - 1 has read P and written O.
-        auto done_before = [&](int j) {
-            const bool done = __all_sync(0xffffffffu, wait_on(sm, smem_u32(&sm.o_done[x]), (j - 1) & 1, err));
-            tc_after();
-            return done;
-        };
-        for (int j = 0; j < tiles; j++) {
-            if (j >= special) {  // (before the scores are there: the output product waits for both halves)
-                ok = __all_sync(0xffffffffu, clear_v(j));
+        unsigned n_s = 0;  // score tiles of x before this item
+        while (next_item()) {
+            const Shape sh(blk, g, QP);
+            const int *nonfinite = &sm.item[(item - 1) % PT_ITEMS].nonfinite;
+            const int nx = x ? sh.n1 : sh.n0, nt = x ? sh.t1 : sh.t0;
+            const int pos = sh.pos0 + x * QP + i;
+            const bool real = i < nx && i < QP;
+            const int whole = max(sh.pos0 + x * QP + 1, 0) / PT_N;  // tiles before this one need no mask
+            float m = -INFINITY, l = 0.f;
+            // The output product of tile j - 1 has read P and written O.
+            auto done_before = [&](int j) {
+                const bool done = wait(smem_u32(&sm.o_done[x]), (n_s + j - 1) & 1);
+                tc_after();
+                return done;
+            };
+            for (int j = 0; j < nt; j++) {
+                ok = wait(smem_u32(&sm.s_full[x]), (n_s + j) & 1);
                 if (!ok) break;
-            }
-            if (j >= nt) continue;  // (the other row tile's last one)
-            ok = wait_on(sm, smem_u32(&sm.s_full[x]), j & 1, err);
-            if (!__all_sync(0xffffffffu, ok)) {
-                ok = false;
-                break;
-            }
-            tc_after();
-            float s[128];
-            tm_ld64(ts, reinterpret_cast<uint32_t *>(s));
-            tm_ld64(ts + 64, reinterpret_cast<uint32_t *>(s + 64));
-            tc_before();
-            bar_arrive(smem_u32(&sm.s_read));
-            if (j >= whole) {
-                const int seen = pos - j * PT_N;  // keys 0 .. seen of this tile
+                tc_after();
+                float s[128];
+                tm_ld64(ts, reinterpret_cast<uint32_t *>(s));
+                tm_ld64(ts + 64, reinterpret_cast<uint32_t *>(s + 64));
+                tc_before();
+                bar_arrive(smem_u32(&sm.s_read));
+                if (j >= whole) {
+                    const int seen = pos - j * PT_N;  // keys 0 .. seen of this tile
 #pragma unroll
-                for (int e = 0; e < 128; e++) s[e] = e <= seen ? s[e] : -INFINITY;
-            }
-            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    for (int e = 0; e < 128; e++) s[e] = e <= seen ? s[e] : -INFINITY;
+                }
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int e = 0; e < 128; e += 8)
+                for (int e = 0; e < 128; e += 8)
 #pragma unroll
-                for (int k = 0; k < 4; k++) mx[k] = max3(mx[k], s[e + 2 * k], s[e + 2 * k + 1]);
-            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-            const bool up = top > m && (m == -INFINITY || (top - m) * c > PT_RAISE);
-            if (__any_sync(0xffffffffu, up)) {
-                const float f = up ? (m == -INFINITY ? 0.f : ex2((m - top) * c)) : 1.f;
-                if (up) m = top;
-                l *= f;
-                if (j > 0) {
-                    ok = done_before(j);
-                    if (!ok) break;
+                    for (int k = 0; k < 4; k++) mx[k] = max3(mx[k], s[e + 2 * k], s[e + 2 * k + 1]);
+                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                const bool up = top > m && (m == -INFINITY || (top - m) * c > PT_RAISE);
+                if (__any_sync(0xffffffffu, up)) {
+                    const float f = up ? (m == -INFINITY ? 0.f : ex2((m - top) * c)) : 1.f;
+                    if (up) m = top;
+                    l *= f;
+                    if (j > 0) {
+                        ok = done_before(j);
+                        if (!ok) break;
 #pragma unroll 1
-                    for (int k = 0; k < 128; k += 32) {
-                        uint32_t o[32];
-                        tm_ld32(to + k, o);
+                        for (int k = 0; k < 128; k += 32) {
+                            uint32_t o[32];
+                            tm_ld32(to + k, o);
 #pragma unroll
-                        for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                        tm_st32(to + k, o);
+                            for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                            tm_st32(to + k, o);
+                        }
                     }
                 }
-            }
-            const float mc = m == -INFINITY ? 0.f : m * c - shift;
-            const uint64_t c2 = pair(c, c), mc2 = pair(-mc, -mc);
-            uint64_t sum[2] = {0ull, 0ull};
+                const float mc = m == -INFINITY ? 0.f : m * c - shift;
+                const uint64_t c2 = pair(c, c), mc2 = pair(-mc, -mc);
+                uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
-            for (int k = 0; k < 128; k += 64) {
-                uint32_t p[32];
+                for (int k = 0; k < 128; k += 64) {
+                    uint32_t p[32];
 #pragma unroll
-                for (int e = 0; e < 64; e += 2) {
-                    const uint64_t x2 = fma2(pair(s[k + e], s[k + e + 1]), c2, mc2);
-                    float p0, p1;
-                    unpair(x2, p0, p1);
-                    p0 = ex2(p0);
-                    p1 = ex2(p1);
-                    sum[(e / 2) & 1] = add2(sum[(e / 2) & 1], pair(p0, p1));
-                    p[e / 2] = T::plain(p0, p1);
+                    for (int e = 0; e < 64; e += 2) {
+                        const uint64_t x2 = fma2(pair(s[k + e], s[k + e + 1]), c2, mc2);
+                        float p0, p1;
+                        unpair(x2, p0, p1);
+                        p0 = ex2(p0);
+                        p1 = ex2(p1);
+                        sum[(e / 2) & 1] = add2(sum[(e / 2) & 1], pair(p0, p1));
+                        p[e / 2] = T::plain(p0, p1);
+                    }
+                    if (k == 0 && j > 0) {
+                        ok = done_before(j);
+                        if (!ok) break;
+                    }
+                    tm_st32(tp + k / 2, p);
                 }
-                if (k == 0 && j > 0) {
-                    ok = done_before(j);
-                    if (!ok) break;
-                }
-                tm_st32(tp + k / 2, p);
-            }
-            {
+                if (!ok) break;
                 float s0, s1;
                 unpair(add2(sum[0], sum[1]), s0, s1);
                 l += s0 + s1;
+                tm_st_wait();
+                tc_before();
+                bar_arrive(smem_u32(&sm.p_full[x]));
             }
+            if (ok && nt > 0) ok = done_before(nt);
             if (!ok) break;
-            tm_st_wait();
-            tc_before();
-            bar_arrive(smem_u32(&sm.p_full[x]));
-        }
-        if (ok && nt > 0) ok = wait_on(sm, smem_u32(&sm.o_done[x]), (nt - 1) & 1, err);
-        if (ok && nt == 0 && tiles > 0) ok = wait_on(sm, smem_u32(&sm.q_full), 0, err);  // (its rows are reused below)
-        ok = __all_sync(0xffffffffu, ok);
-        if (ok && nx > 0) {
-            tc_after();
-            const float inv = l > 0.f ? 1.0f / l : (isnan(l) ? l : 0.f);
-            const bool fix = sm.nonfinite != 0;  // (written before the products that o_done waited for)
-            // rows go through the row tile's Q (all its scores are done): a row's 16
-            // pieces of 16 bytes, exchanged by the row's number so that neither side
-            // has bank conflicts, leave in whole rows
-            unsigned char *stage = sm.q[x] + (warp & 3) * 32 * 256;
-            const unsigned inv_g = (65536u + G - 1) / G;  // r / G = r * inv_g >> 16 for r < 128
-            const float scale_o = l > 0.f || isnan(l) ? inv : 0.f;
-            for (int part = 0; part < (a.lo ? 2 : 1); part++) {  // (hi, then lo of a bf16 pair)
-                auto word = [&](uint32_t x, uint32_t y) {
-                    const float u = __uint_as_float(x), v = __uint_as_float(y);
-                    return a.lo ? QdbBf16::plain(pair_part(u, part), pair_part(v, part)) : T::plain(u, v);
-                };
+            if (nx > 0) {
+                const float scale_o = l > 0.f ? 1.0f / l : (isnan(l) ? l : 0.f);
+                const bool fix = *reinterpret_cast<const volatile int *>(nonfinite) != 0;  // (written before the products)
+                // rows leave through shared memory, 64 dims at a time: a row's 8 pieces of
+                // 16 bytes, exchanged by the row's number so that neither side has bank
+                // conflicts, go out together
+                for (int part = 0; part < (PAIR ? 2 : 1); part++) {  // (hi, then lo of a bf16 pair)
+                    auto word = [&](uint32_t y, uint32_t z) {
+                        const float u = __uint_as_float(y), v = __uint_as_float(z);
+                        return PAIR ? QdbBf16::plain(pair_part(u, part), pair_part(v, part)) : T::plain(u, v);
+                    };
 #pragma unroll 1
-                for (int k = 0; k < 128; k += 64) {
-                    uint32_t o[64];
-                    if (nt > 0) {
-                        tm_ld64(to + k, o);
-                    } else {
+                    for (int k = 0; k < 128; k += 64) {
+                        uint32_t o[64];
+                        if (nt > 0) {
+                            tm_ld64(to + k, o);
+                        } else {
 #pragma unroll
-                        for (int e = 0; e < 64; e++) o[e] = 0u;
-                    }
-#pragma unroll
-                    for (int e = 0; e < 64; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * scale_o);
-                    if (fix && real)  // non-finite values were left out of the products: add those this row sees
-                        for (int key = special * PT_N; key <= pos; key++) {
-                            const int page = paged_page(a.kv, a.bt, blk.b, key >> a.kv.page_shift);
-                            if (page < 0) continue;
-                            const uint16_t *v = a.kv.v + page * a.kv.page_stride + g * a.kv.head_stride +
-                                                (key & ((1 << a.kv.page_shift) - 1)) * a.kv.pos_stride + k;
-#pragma unroll
-                            for (int e = 0; e < 64; e++) {
-                                const float y = T::lo(v[e]);
-                                if (!isfinite(y)) o[e] = __float_as_uint(__uint_as_float(o[e]) + y);
-                            }
+                            for (int e = 0; e < 64; e++) o[e] = 0u;
                         }
 #pragma unroll
-                    for (int e = 0; e < 64; e += 8)
-                        *reinterpret_cast<uint4 *>(stage + lane * 256 + ((((k + e) / 8) ^ (lane & 7)) << 4)) =
-                            make_uint4(word(o[e], o[e + 1]), word(o[e + 2], o[e + 3]), word(o[e + 4], o[e + 5]),
-                                       word(o[e + 6], o[e + 7]));
+                        for (int e = 0; e < 64; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * scale_o);
+                        if (fix && real)  // non-finite values were left out of the products: add those this row sees
+                            for (int key = sh.special * PT_N; key <= pos; key++) {
+                                const int page = paged_page(a.kv, a.bt, sh.b, key >> a.kv.page_shift);
+                                if (page < 0) continue;
+                                const uint16_t *v = a.kv.v + page * a.kv.page_stride + g * a.kv.head_stride +
+                                                    (key & ((1 << a.kv.page_shift) - 1)) * a.kv.pos_stride + k;
+#pragma unroll
+                                for (int e = 0; e < 64; e++) {
+                                    const float y = T::lo(v[e]);
+                                    if (!isfinite(y)) o[e] = __float_as_uint(__uint_as_float(o[e]) + y);
+                                }
+                            }
+
+                        if (real) {
+                            uint16_t *dst = (part ? a.lo : a.out) + (size_t)(sh.row0 + x * QP + i) * a.out_stride +
+                                            ((size_t)g * G + r - i * G) * QDB_HD + k;
+#pragma unroll
+                            for (int e = 0; e < 64; e += 8)
+                                *reinterpret_cast<uint4 *>(dst + e) =
+                                    make_uint4(word(o[e], o[e + 1]), word(o[e + 2], o[e + 3]), word(o[e + 4], o[e + 5]),
+                                               word(o[e + 6], o[e + 7]));
+                        }
+                        __syncwarp();  // (the rows have been read)
+                    }
                 }
-                __syncwarp();
-#pragma unroll 4
-                for (int e = 0; e < 32; e += 2) {  // two rows at a time
-                    const int q = e + (lane >> 4), rr = 32 * (warp & 3) + q, ii = (int)((unsigned)rr * inv_g >> 16);
-                    if (ii >= nx || ii >= QP) continue;
-                    uint16_t *dst = (part ? a.lo : a.out) + (size_t)(blk.row0 + x * QP + ii) * a.out_stride + ((size_t)g * G + rr - ii * G) * QDB_HD;
-                    *reinterpret_cast<uint4 *>(dst + (lane & 15) * 8) =
-                        *reinterpret_cast<const uint4 *>(stage + q * 256 + (((lane & 15) ^ (q & 7)) << 4));
-                }
-                __syncwarp();  // (the rows have been read)
             }
+            tc_before();  // (O has been read: before the next item's first weights are announced)
+            n_s += nt;
+            item_done();
         }
     } else if (warp < 10) {
         // ------------------------------------------------ products: warp 8 the scores, warp 9 the outputs
         // (the whole warp runs this together, with values that are the same in all
         // lanes, so that they stay in uniform registers, where the products' operands
         // have to be; one lane issues)
-        const int T0 = __shfl_sync(0xffffffffu, t0, 0), T1 = __shfl_sync(0xffffffffu, t1, 0), TT = max(T0, T1);
-        const int part = __shfl_sync(0xffffffffu, special, 0);
         const uint32_t tmu = __shfl_sync(0xffffffffu, tm, 0);
-        if (TT > 0) {
-            bool ok = true;
-            const bool scores_warp = warp == 8, leader = elect();  // (a commit covers its own thread's products)
-            const uint64_t q_desc = op_desc(smem_u32(sm.q[0]), 16), k_desc = op_desc(smem_u32(sm.k[0]), 16),
-                           v_desc = op_desc(smem_u32(sm.v[0]), PT_HALF);
-            constexpr uint64_t tile = PT_TILE >> 4;
-            auto scores = [&](int x, int j) {  // S = Q_x K_j^T
-                const uint64_t q = q_desc + x * tile, k = k_desc + (uint32_t)(j % PT_KS) * tile;
-                if (leader) {
-                    mma_ss<false>(tmu, q, k, op_kind<T>(false));
+        const bool scores_warp = warp == 8, leader = elect();  // (a commit covers its own thread's products)
+        const uint64_t q_desc = op_desc(smem_u32(sm.q[0]), 16), k_desc = op_desc(smem_u32(sm.k[0]), 16),
+                       v_desc = op_desc(smem_u32(sm.v[0]), PT_HALF);
+        constexpr uint64_t tile = PT_TILE >> 4;
+        auto scores = [&](int x, unsigned st) {  // S = Q_x K^T
+            const uint64_t q = q_desc + x * tile, k = k_desc + st * tile;
+            if (leader) {
+                mma_ss<false>(tmu, q, k, op_kind<T>(false));
 #pragma unroll
-                    for (int e = 1; e < 8; e++) {
-                        const uint64_t at = ((e >> 2) * PT_HALF + (e & 3) * 32) >> 4;
-                        mma_ss<true>(tmu, q + at, k + at, op_kind<T>(false));
-                    }
-                    commit(smem_u32(&sm.s_full[x]));
+                for (int e = 1; e < 8; e++) {
+                    const uint64_t at = ((e >> 2) * PT_HALF + (e & 3) * 32) >> 4;
+                    mma_ss<true>(tmu, q + at, k + at, op_kind<T>(false));
                 }
-                __syncwarp();
-            };
-            auto output = [&](int x, int j) {  // O_x += P_x V_j
-                const uint64_t v = v_desc + (uint32_t)(j % PT_VS) * tile;
-                const uint32_t d = tmu + 256 + x * 128, p = tmu + 128 + x * 64;
-                if (leader) {
-                    if (j > 0) mma_ts<true>(d, p, v, op_kind<T>(true));
-                    else mma_ts<false>(d, p, v, op_kind<T>(true));
+                commit(smem_u32(&sm.s_full[x]));
+            }
+            __syncwarp();
+        };
+        auto output = [&](int x, unsigned st, bool more) {  // O_x (+)= P_x V
+            const uint64_t v = v_desc + st * tile;
+            const uint32_t d = tmu + 256 + x * 128, p = tmu + 128 + x * 64;
+            if (leader) {
+                if (more) mma_ts<true>(d, p, v, op_kind<T>(true));
+                else mma_ts<false>(d, p, v, op_kind<T>(true));
 #pragma unroll
-                    for (int e = 1; e < 8; e++) mma_ts<true>(d, p + e * 8, v + e * (2048 >> 4), op_kind<T>(true));
-                    commit(smem_u32(&sm.o_done[x]));
-                }
-                __syncwarp();
-            };
-            auto wait = [&](uint32_t bar, unsigned parity) { return __all_sync(0xffffffffu, wait_on(sm, bar, parity, err)); };
-            // the tiles in the order 0(0) 1(0) 0(1) 1(1) ...; those a row tile does
-            // not need are passed over
-            int n = 0;
-            if (scores_warp) ok = wait(smem_u32(&sm.q_full), 0);
-            for (int j = 0; j < TT && ok; j++) {
-                if (scores_warp) {
-                    ok = wait(smem_u32(&sm.k_full[j % PT_KS]), (j / PT_KS) & 1);
-                } else if (j < part) {
-                    ok = wait(smem_u32(&sm.v_full[j % PT_VS]), (j / PT_VS) & 1);
-                } else {  // V_j, which some row sees only in part, landed and was cleared
-                    ok = wait(smem_u32(&sm.v_clean[j - part]), 0);
+                for (int e = 1; e < 8; e++) mma_ts<true>(d, p + e * 8, v + e * (2048 >> 4), op_kind<T>(true));
+                commit(smem_u32(&sm.o_done[x]));
+            }
+            __syncwarp();
+        };
+        unsigned n_tile = 0, n_part = 0, n_q = 0, n_s = 0, n_p0 = 0, n_p1 = 0;
+        while (next_item()) {
+            const Shape sh(blk, g, QP);
+            const int T0 = __shfl_sync(0xffffffffu, sh.t0, 0), T1 = __shfl_sync(0xffffffffu, sh.t1, 0), TT = max(T0, T1);
+            const int part = __shfl_sync(0xffffffffu, sh.special, 0);
+            item_done();
+            if (TT == 0) continue;
+            if (scores_warp) ok = wait(smem_u32(&sm.q_full), n_q++ & 1);
+            // row tiles 0 and 1 in turn, tile after tile
+            for (int j = 0; j < TT && ok; j++, n_tile++) {
+                const unsigned st = n_tile % (scores_warp ? PT_KS : PT_VS), use = n_tile / (scores_warp ? PT_KS : PT_VS);
+                ok = wait(smem_u32(scores_warp ? &sm.k_full[st] : &sm.v_full[st]), use & 1);
+                if (!scores_warp && ok && j >= part) {  // warp 11 clears the other half
+                    clear_v(st, 0, min(sh.end - j * PT_N, PT_N));
+                    ok = wait(smem_u32(&sm.v_clean[n_part % PT_PART]), (n_part / PT_PART) & 1);
+                    n_part++;
                 }
                 for (int x = 0; x < 2 && ok; x++) {
                     if (j >= (x ? T1 : T0)) continue;
                     if (scores_warp) {  // (the scores before have been read)
-                        if (n) ok = wait(smem_u32(&sm.s_read), (n - 1) & 1);
+                        if (n_s) ok = wait(smem_u32(&sm.s_read), (n_s - 1) & 1);
+                        n_s++;
                     } else {
-                        ok = wait(smem_u32(&sm.p_full[x]), j & 1);
+                        ok = wait(smem_u32(&sm.p_full[x]), (x ? n_p1++ : n_p0++) & 1);
                     }
                     if (!ok) break;
                     tc_after();
-                    if (scores_warp) scores(x, j);
-                    else output(x, j);
-                    n++;
+                    if (scores_warp) scores(x, st);
+                    else output(x, st, j > 0);
                 }
-                if (ok && leader) commit(smem_u32(scores_warp ? &sm.k_empty[j % PT_KS] : &sm.v_empty[j % PT_VS]));
+                if (ok && leader) commit(smem_u32(scores_warp ? &sm.k_empty[st] : &sm.v_empty[st]));
                 __syncwarp();
             }
-            if (!ok && n) {  // given up: the products in flight end before the CTA does
-                if (leader) commit(smem_u32(&sm.drain[warp - 8]));
-                __syncwarp();
-                bar_wait(smem_u32(&sm.drain[warp - 8]), 0, err);
-            }
+            if (!ok) break;
+            if (scores_warp && leader) commit(smem_u32(&sm.q_empty));
+            __syncwarp();
         }
+        // the products and commits in flight end before the CTA does
+        if (leader) commit(smem_u32(&sm.drain[warp - 8]));
         __syncwarp();
-    } else if (tiles > 0) {
-        // ------------------------------------------------ copies: warp 10 Q and K, warp 11 V
-        const bool is_v = warp == 11;
+        bar_wait(smem_u32(&sm.drain[warp - 8]), 0, err);
+        __syncwarp();
+    } else {
+        // ------------------------------------------------ copies: warp 10 Q and K (and the items), warp 11 V
+        const bool is_v = warp == 11, leader = elect();
         const int rows = min(1 << a.kv.page_shift, PT_N), pieces = PT_N / rows, S = is_v ? PT_VS : PT_KS;
         unsigned long long *full = is_v ? sm.v_full : sm.k_full, *empty = is_v ? sm.v_empty : sm.k_empty;
-        unsigned char *ring = is_v ? sm.v[0] : sm.k[0];
+        const uint32_t ring = smem_u32(is_v ? sm.v[0] : sm.k[0]);
         const CUtensorMap *map = is_v ? &mv : &mk;
-        auto look_up = [&](int j) {  // this lane's page of tile j
-            const int key = j * PT_N + lane * rows;
-            if (lane >= pieces || key >= end) return -1;
-            const int p = paged_page(a.kv, a.bt, blk.b, key >> a.kv.page_shift);
-            return p < 0 ? a.kv.n_pages : p;  // outside the pool: recorded, reads as zeros
-        };
-        int page = look_up(0);
-        if (!is_v && lane == 0) {
-            bar_expect(smem_u32(&sm.q_full), (n1 > 0 ? 4u : 2u) * 128u * G * QP);
-            for (int x = 0; x < (n1 > 0 ? 2 : 1); x++)
-                for (int half = 0; half < 2; half++)
-                    asm volatile(
-                        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, "
-                        "{%2, %3, %4, %5}], [%6];" ::"r"(smem_u32(sm.q[x]) + half * PT_HALF),
-                        "l"(&mq), "r"(0), "r"(half), "r"(g * G), "r"(blk.row0 + x * QP), "r"(smem_u32(&sm.q_full))
-                        : "memory");
-        }
-        __syncwarp();
-        bool ok = true;
-        int sent = 0;
-        for (int j = 0; j < tiles; j++) {
-            const int st = j % S, n = min(pieces, (end - j * PT_N + rows - 1) / rows);
-            const int after = j + 1 < tiles ? look_up(j + 1) : -1;  // (not waited for before it is needed)
-            if (j >= S) ok = __all_sync(0xffffffffu, wait_on(sm, smem_u32(&empty[st]), ((j / S) & 1) ^ 1, err));
-            if (!ok) break;
-            // (V of a tile seen in part lands on a barrier of its own, which the
-            // clearing warps wait for, and which has one phase only)
-            const uint32_t bar = smem_u32(is_v && j >= special ? &sm.v_part[j - special] : &full[st]);
-            if (lane == 0) bar_expect(bar, (uint32_t)n * rows * 256u);
-            __syncwarp();
-            if (page >= 0) {
-                const uint32_t dst = smem_u32(ring) + st * PT_TILE + lane * rows * 128;
-                const int slot = (j * PT_N + lane * rows) & ((1 << a.kv.page_shift) - 1);
-#pragma unroll
-                for (int half = 0; half < 2; half++) load_half_page(dst + half * PT_HALF, map, slot, half, g, page, bar);
+        unsigned n_tile = 0, n_q = 0, n_part = 0;
+        // The CTA's items: its own number, then those of CTAs that have not been
+        // launched yet, taken from the launch queue until none is left. It asks for
+        // the next one two tiles before this one's end: at once, a CTA with a heavy
+        // item would keep a second one from those that will be free before it.
+        int number = blockIdx.x;
+        unsigned asked = 0, answered = 0;
+        auto ask = [&] {
+            if (leader) {
+                fence_async();  // (the last answer has been read)
+                bar_expect(smem_u32(&sm.stolen_bar), 16);
+                asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                                 smem_u32(sm.stolen)),
+                             "r"(smem_u32(&sm.stolen_bar))
+                             : "memory");
             }
             __syncwarp();
-            page = after;
-            sent = j + 1;
+            asked++;
+        };
+        auto answer = [&] {  // the number taken, or -1: none is left
+            ok = wait(smem_u32(&sm.stolen_bar), answered++ & 1);
+            if (!ok) return -1;
+            const volatile uint64_t *w = sm.stolen;
+            const uint64_t lo = w[0], hi = w[1];
+            uint32_t got, x = 0;
+            asm volatile(
+                "{ .reg .b128 r; .reg .pred p; mov.b128 r, {%2, %3};\n\t"
+                "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+                "selp.u32 %0, 1, 0, p;\n\tmov.u32 %1, 0;\n\t"
+                "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r; }"
+                : "=r"(got), "=r"(x)
+                : "l"(lo), "l"(hi));
+            __syncwarp();
+            return got ? (int)x : -1;
+        };
+        bool first = true;
+        auto announce = [&]() -> bool {  // the next block that has rows
+            for (;; first = false) {
+                if (!first && number >= 0) {
+                    if (asked == answered) ask();
+                    number = answer();
+                    if (!ok) return false;
+                }
+                Block k{0, 0, 0, 0, false};
+                if (number >= 0) {
+                    k = find_block(a, 2 * QP, number / Hkv, lane);
+                    if (!k.any) continue;
+                }
+                const int s = item % PT_ITEMS;
+                if (item >= PT_ITEMS) ok = wait(smem_u32(&sm.item_empty[s]), ((item / PT_ITEMS) & 1) ^ 1);
+                if (!ok) return false;
+                blk = k;
+                g = number >= 0 ? number % Hkv : 0;
+                if (lane == 0) {
+                    sm.item[s] = Item{k, g, 0};
+                    bar_arrive(smem_u32(&sm.item_full[s]));
+                }
+                __syncwarp();
+                item++;
+                first = false;
+                return k.any;
+            }
+        };
+        while (is_v ? next_item() : announce()) {
+            const Shape sh(blk, g, QP);
+            auto look_up = [&](int j) {  // this lane's page of tile j
+                const int key = j * PT_N + lane * rows;
+                if (lane >= pieces || key >= sh.end) return -1;
+                const int p = paged_page(a.kv, a.bt, sh.b, key >> a.kv.page_shift);
+                return p < 0 ? a.kv.n_pages : p;  // outside the pool: recorded, reads as zeros
+            };
+            if (sh.tiles == 0) {
+                if (is_v) item_done();
+                continue;
+            }
+            int page = look_up(0);
+            const int end = __shfl_sync(0xffffffffu, sh.end, 0), head = __shfl_sync(0xffffffffu, g, 0);
+            for (int j = 0; j < sh.tiles; j++) {
+                const int n = min(pieces, (end - j * PT_N + rows - 1) / rows), slot = (j * PT_N) & ((1 << a.kv.page_shift) - 1);
+                const int after = j + 1 < sh.tiles ? look_up(j + 1) : -1;  // (not waited for before it is needed)
+                const unsigned st = n_tile % S;
+                if (n_tile >= (unsigned)S) ok = wait(smem_u32(&empty[st]), ((n_tile / S) & 1) ^ 1);
+                if (!ok) break;
+                // pieces one after the other, all operands the same in every lane
+                const uint32_t dst = ring + st * PT_TILE, bar = smem_u32(&full[st]);
+                if (leader) bar_expect(bar, (uint32_t)n * rows * 256u);
+                for (int p = 0; p < n; p++) {
+                    const int pg = __shfl_sync(0xffffffffu, page, p);
+                    if (leader) {
+                        load_half_page(dst + p * rows * 128, map, slot, 0, head, pg, bar);
+                        load_half_page(dst + p * rows * 128 + PT_HALF, map, slot, 1, head, pg, bar);
+                    }
+                }
+                __syncwarp();
+                n_tile++;
+                page = after;
+                if (is_v) continue;
+                if (j == 0) {  // Q, once the item before has no more use for its rows
+                    if (n_q) ok = wait(smem_u32(&sm.q_empty), (n_q - 1) & 1);
+                    if (!ok) break;
+                    n_q++;
+                    if (leader) {
+                        bar_expect(smem_u32(&sm.q_full), (sh.n1 > 0 ? 4u : 2u) * 128u * G * QP);
+                        for (int x = 0; x < (sh.n1 > 0 ? 2 : 1); x++)
+                            for (int half = 0; half < 2; half++)
+                                asm volatile(
+                                    "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], "
+                                    "[%1, {%2, %3, %4, %5}], [%6];" ::"r"(smem_u32(sm.q[x]) + half * PT_HALF),
+                                    "l"(&mq), "r"(0), "r"(half), "r"(head * G), "r"(sh.row0 + x * QP),
+                                    "r"(smem_u32(&sm.q_full))
+                                    : "memory");
+                    }
+                    __syncwarp();
+                }
+                if (j == max(sh.tiles - 2, 0)) ask();
+            }
+            if (!ok) break;
+            if (is_v) {
+                // (all of the item's tiles are on their way: those seen in part are its last
+                // ones, no more than the ring holds, so none waits for another's clearing)
+                for (int j = sh.special; j < sh.tiles; j++, n_part++) {
+                    const unsigned k = n_tile - sh.tiles + j;
+                    ok = wait(smem_u32(&full[k % S]), (k / S) & 1);
+                    if (!ok) break;
+                    clear_v(k % S, 1, min(end - j * PT_N, PT_N));
+                    if (leader) bar_arrive(smem_u32(&sm.v_clean[n_part % PT_PART]));
+                }
+                if (!ok) break;
+                item_done();
+            }
         }
-        if (!ok && lane == 0) {  // given up: the copies in flight land first
-            if (!is_v) bar_wait(smem_u32(&sm.q_full), 0, err);
-            for (int j = max(0, sent - S); j < sent; j++)
-                bar_wait(smem_u32(is_v && j >= special ? &sm.v_part[j - special] : &full[j % S]),
-                         is_v && j >= special ? 0u : (unsigned)(j / S) & 1u, err);
+        if (!ok) {  // given up: what is in flight lands first
+            if (asked > answered) bar_wait(smem_u32(&sm.stolen_bar), answered & 1, err);
+            if (n_q) bar_wait(smem_u32(&sm.q_full), (n_q - 1) & 1, err);
+            for (unsigned k = n_tile > (unsigned)S ? n_tile - S : 0; k < n_tile; k++)
+                bar_wait(smem_u32(&full[k % S]), (k / S) & 1, err);
         }
         __syncwarp();
     }
@@ -596,16 +721,16 @@ int query_map(CUtensorMap *map, const QdbPagedAttnArgs &a, int type, int G) {
                            (uint32_t)(128 / G));
 }
 
-template <typename T>
+template <typename T, bool PAIR>
 cudaError_t launch(const CUtensorMap &mq, const CUtensorMap &mk, const CUtensorMap &mv, const QdbPagedAttnArgs &a,
                    cudaStream_t st) {
     const size_t smem = sizeof(PromptSmem) + 1024;
-    cudaError_t e = cudaFuncSetAttribute(prompt_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    cudaError_t e = cudaFuncSetAttribute(prompt_kernel<T, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
     const int G = a.heads / a.kv.kv_heads, bq = 2 * (128 / G);
     const long long blocks = a.bt.q_starts ? (long long)a.bt.rows / bq + a.bt.n_seqs : a.bt.n_seqs;
     if (blocks * a.kv.kv_heads > 2147483647ll) return cudaErrorInvalidConfiguration;
-    return pdl_launch(prompt_kernel<T>, dim3((unsigned)(blocks * a.kv.kv_heads)), dim3(PT_THREADS), smem, st, mq, mk, mv, a);
+    return pdl_launch(prompt_kernel<T, PAIR>, dim3((unsigned)(blocks * a.kv.kv_heads)), dim3(PT_THREADS), smem, st, mq, mk, mv, a);
 }
 
 }  // namespace
@@ -616,5 +741,7 @@ cudaError_t qdb_launch_paged_prompt(const QdbPagedAttnArgs &a, int type, cudaStr
     if (query_map(&mq, a, type, a.heads / a.kv.kv_heads) || qdb_paged_map(&mk, a.kv.k, a.kv, type, rows, 1) ||
         qdb_paged_map(&mv, a.kv.v, a.kv, type, rows, 1))
         return cudaErrorInvalidValue;
-    return type == QDB_TYPE_F16 ? launch<QdbHalf>(mq, mk, mv, a, st) : launch<QdbBf16>(mq, mk, mv, a, st);
+    if (a.lo)
+        return type == QDB_TYPE_F16 ? launch<QdbHalf, true>(mq, mk, mv, a, st) : launch<QdbBf16, true>(mq, mk, mv, a, st);
+    return type == QDB_TYPE_F16 ? launch<QdbHalf, false>(mq, mk, mv, a, st) : launch<QdbBf16, false>(mq, mk, mv, a, st);
 }
