@@ -435,14 +435,16 @@ typedef struct {
  * cache's type. f16 stores saturate at +-65504. row_stride / q_stride: elements
  * between rows (0 = contiguous), multiples of 16 bytes. A row at a negative
  * position (more rows than kv_lens) is left out. Up to 16 query heads per key
- * head. A position must not occur twice in one call. */
+ * head. A position must not occur twice in one call, and the rows, q_out and the
+ * cache must not overlap. */
 int qdb_paged_append(const qdb_paged_kv *kv, const qdb_paged_batch *batch, const void *qkv, int src_type,
                      long long row_stride, int heads, const float *q_norm, const float *k_norm, float eps,
                      const float *rope, int rope_len, void *q_out, long long q_stride, void *stream);
 
 /* Scratch of qdb_paged_decode on `device` (about 3 MB, allocated and cleared
  * here). One call uses it at a time: calls that may overlap on the GPU (two
- * streams, two graphs replayed at once) need one each. NULL on error. */
+ * streams, two graphs replayed at once) need one each. After a call whose err
+ * words report a wait that ran out ({1, ..}), make a new one. NULL on error. */
 typedef struct qdb_paged_workspace qdb_paged_workspace;
 qdb_paged_workspace *qdb_paged_workspace_create(int device);
 void qdb_paged_workspace_free(qdb_paged_workspace *ws);
@@ -452,7 +454,8 @@ void qdb_paged_workspace_free(qdb_paged_workspace *ws);
  * [rows, heads * 128] in the cache's type, q_stride / out_stride elements
  * between rows (0 = contiguous, multiples of 8); scale 0 = 1/sqrt(128). Query
  * head h reads key head h / (heads / kv_heads); at most 16 query heads per key
- * head. A sequence of length 0 gives a row of zeros. The page tables together
+ * head. A sequence of length 0 gives a row of zeros. q, out and the cache must
+ * not overlap. The page tables together
  * may span up to n_seqs * table_stride * page_size * kv_heads = 2^35. */
 int qdb_paged_decode(const qdb_paged_kv *kv, const qdb_paged_batch *batch, const void *q, long long q_stride,
                      int heads, float scale, void *out, long long out_stride, qdb_paged_workspace *ws, void *stream);

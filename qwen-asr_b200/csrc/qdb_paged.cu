@@ -1,9 +1,11 @@
-// qdb_paged.cu - paged KV cache: rotation and append of new positions, and
-// attention over the pages.
+// qdb_paged.cu - paged KV cache: rotation and append of new positions; tensor
+// maps of the pages; the C entry points of the paged operators and their checks.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <math.h>
 #include <stdio.h>
+
+#include <new>
 
 #include "qdb_kernels.h"
 #include "qdb_paged.cuh"
@@ -163,6 +165,12 @@ cudaError_t qdb_decode_scratch_alloc(int device, QdbDecodeScratch *s) {
     if (e == cudaSuccess) e = cudaMalloc((void **)&s->cnt, sizeof(unsigned) * s->ctas);
     if (e == cudaSuccess) e = cudaMemset(s->cnt, 0, sizeof(unsigned) * s->ctas);
     if (e == cudaSuccess) e = cudaDeviceSynchronize();
+    if (e != cudaSuccess) {  // all or nothing
+        cudaFree(s->part);
+        cudaFree(s->ml);
+        cudaFree(s->cnt);
+        *s = {};
+    }
     return e;
 }
 
@@ -224,6 +232,11 @@ static bool on_device(const void *p, int dev, const char *what, char *msg, size_
 
 int qdb_check_device_ptrs(const char *fn, const QdbNamedPtr *ps, int n) {
     char msg[256], full[320];
+    for (int i = 0; i < n; i++)
+        if ((uintptr_t)ps[i].p % ps[i].align) {
+            snprintf(full, sizeof(full), "%s: %s is not aligned to %d bytes", fn, ps[i].name, ps[i].align);
+            return qdb_set_error(full);
+        }
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) {
@@ -316,7 +329,11 @@ extern "C" qdb_paged_workspace *qdb_paged_workspace_create(int device) {
         qdb_set_error(m);
         return nullptr;
     }
-    qdb_paged_workspace *ws = new qdb_paged_workspace{device, {}};
+    qdb_paged_workspace *ws = new (std::nothrow) qdb_paged_workspace{device, {}};
+    if (!ws) {
+        qdb_set_error("qdb_paged_workspace_create: out of memory");
+        return nullptr;
+    }
     int before = 0;
     cudaGetDevice(&before);
     cudaError_t e = cudaSetDevice(device);

@@ -189,11 +189,13 @@ int qdb_paged_map(CUtensorMap *map, const void *pool, const QdbPagedKV &kv, int 
 int qdb_encode_map4(CUtensorMap *map, const void *q, int type, uint64_t heads, uint64_t rows, uint64_t row_stride,
                     uint32_t box_heads, uint32_t box_rows);
 
-// ---- host checks: refuses host pointers and pointers of another device than
-// the current one (null pointers are left to the caller). 0 = ok.
+// ---- host checks: refuses misaligned pointers, host pointers and pointers of
+// another device than the current one (null pointers are left to the caller).
+// 0 = ok.
 struct QdbNamedPtr {
     const void *p;
     const char *name;
+    int align = 4;
 };
 int qdb_check_device_ptrs(const char *fn, const QdbNamedPtr *ps, int n);
 

@@ -435,9 +435,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
             if (nx > 0) {
                 const float scale_o = l > 0.f ? 1.0f / l : (isnan(l) ? l : 0.f);
                 const bool fix = *reinterpret_cast<const volatile int *>(nonfinite) != 0;  // (written before the products)
-                // rows leave through shared memory, 64 dims at a time: a row's 8 pieces of
-                // 16 bytes, exchanged by the row's number so that neither side has bank
-                // conflicts, go out together
+                // a thread stores its own row, 64 dims at a time (passing rows through shared
+                // memory for full 128-byte stores took as long)
                 for (int part = 0; part < (PAIR ? 2 : 1); part++) {  // (hi, then lo of a bf16 pair)
                     auto word = [&](uint32_t y, uint32_t z) {
                         const float u = __uint_as_float(y), v = __uint_as_float(z);
@@ -466,7 +465,6 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                                     if (!isfinite(y)) o[e] = __float_as_uint(__uint_as_float(o[e]) + y);
                                 }
                             }
-
                         if (real) {
                             uint16_t *dst = (part ? a.lo : a.out) + (size_t)(sh.row0 + x * QP + i) * a.out_stride +
                                             ((size_t)g * G + r - i * G) * QDB_HD + k;
@@ -476,7 +474,6 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                                     make_uint4(word(o[e], o[e + 1]), word(o[e + 2], o[e + 3]), word(o[e + 4], o[e + 5]),
                                                word(o[e + 6], o[e + 7]));
                         }
-                        __syncwarp();  // (the rows have been read)
                     }
                 }
             }

@@ -11,6 +11,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <new>
 
 #ifndef QDB_AR_ITERS
 #define QDB_AR_ITERS 8  // 8-key steps per warp of a batched-decode attention unit
@@ -657,7 +658,8 @@ extern "C" qdb_pool *qdb_pool_create(qdb_model *m, int n_pages, int page_size) {
     // (positions are ints)
     if (n_pages <= 0 || n_pages > (0x7fffffff >> shift)) { fail("a pool of %d pages", n_pages); return nullptr; }
     if (set_dev(m)) return nullptr;
-    qdb_pool *p = new qdb_pool();
+    qdb_pool *p = new (std::nothrow) qdb_pool();
+    if (!p) { fail("out of memory"); return nullptr; }
     p->m = m;
     p->n_pages = n_pages;
     p->page_shift = shift;
@@ -698,7 +700,8 @@ extern "C" int qdb_pool_free_pages(const qdb_pool *p) { return p && p->m ? (int)
 extern "C" qdb_session *qdb_session_create_paged(qdb_pool *p, int initial_positions) {
     g_err.clear();
     if (!p || !p->m) { fail("pool missing, or its model has been freed"); return nullptr; }
-    qdb_session *s = new qdb_session();
+    qdb_session *s = new (std::nothrow) qdb_session();
+    if (!s) { fail("out of memory"); return nullptr; }
     s->m = p->m;
     s->pool = p;
     if (initial_positions > 0 && qdb_session_reserve(s, initial_positions)) {
@@ -977,9 +980,14 @@ struct PagedCall {
 static int paged_call(qdb_model *m, qdb_session *const *ss, int n, const int *lens, const int *ends, bool one_row,
                       int rows, const int *step, std::vector<int> &host, PagedCall *pc) {
     RowScratch &r = m->rs;
-    size_t width = 1;  // a power of two: captured steps bake it in
-    for (int i = 0; i < n; i++)
+    size_t width = 1, all = 0;  // width: a power of two, captured steps bake it in
+    for (int i = 0; i < n; i++) {
         while (width < ss[i]->pages.size()) width *= 2;
+        all += ss[i]->pages.size();
+    }
+    // (the one-token attention numbers the rows' tiles of 16 positions)
+    if (one_row && (all << ss[0]->pool->page_shift >> 4) * m->cfg.kv_heads >= (1u << 31))
+        return fail("%d rows over %zu pages are too many positions for one call", n, all);
     host.assign((size_t)n + 1 + n + width * n, 0);
     for (int i = 0; i < n; i++) {
         host[i + 1] = host[i] + (one_row ? 1 : lens[i]);
@@ -1180,6 +1188,8 @@ static int check_rows_err(qdb_model *m) {
     CK(cudaMemcpy(ev, m->rs.err, sizeof(ev), cudaMemcpyDeviceToHost));
     if (ev[0]) {
         cudaMemset(m->rs.err, 0, sizeof(ev));
+        // (a part that never came leaves a counter of the joins behind)
+        if (m->rs.pdec.cnt) cudaMemset(m->rs.pdec.cnt, 0, sizeof(unsigned) * m->rs.pdec.ctas);
         return fail("device error code %d in a tensor-core GEMM (%s)", ev[0],
                     ev[0] == QDB_ERR_BOUNDS ? "an access refused by a bounds check" : "a bounded wait ran out");
     }
@@ -1218,7 +1228,7 @@ static int prefill_rows(qdb_session *const *ss, int nsess, const int *lens, cons
     RowScratch &r = m->rs;
     if (ss[0]->pool) {
         std::vector<int> ends(nsess), host;
-        for (int i = 0; i < nsess; i++) ends[i] = starts[i] + lens[i];
+        for (int i = 0; i < nsess; i++) ends[i] = lens[i] ? starts[i] + lens[i] : 0;  // (no rows: no position either)
         PagedCall pc;
         CK(cudaMemcpyAsync(r.X, embeds, (size_t)T * m->cfg.hidden * 4,
                            device_ptr ? cudaMemcpyDeviceToDevice : cudaMemcpyHostToDevice, m->st));
@@ -1589,7 +1599,10 @@ extern "C" int qdb_forward_batch(qdb_session *const *sessions, int n, const floa
         return std::vector<const void *>{(const void *)(intptr_t)n, (const void *)(intptr_t)S,
                                          (const void *)(intptr_t)m->mask_eos, m->rope, r.X, r.XH, r.XL, r.QKV, r.Q,
                                          r.ATT, r.ACT, r.LOG, r.part, r.acnt, r.GU, r.tok, r.err, r.rowkv, r.amax,
-                                         pc.pool, pc.pool ? pc.pool->k : nullptr, r.pmeta,
+                                         // (a new pool may get a freed one's addresses)
+                                         pc.pool, pc.pool ? pc.pool->k : nullptr, pc.pool ? pc.pool->v : nullptr,
+                                         (const void *)(intptr_t)(pc.pool ? pc.pool->n_pages : 0),
+                                         (const void *)(intptr_t)(pc.pool ? pc.pool->page_shift : 0), r.pmeta,
                                          (const void *)(intptr_t)pc.bt.table_stride, r.pdec.part};
     };
     const std::vector<const void *> key = graph_key();

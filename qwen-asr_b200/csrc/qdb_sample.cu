@@ -880,8 +880,7 @@ extern "C" int qdb_sample(const void *logits, int type, long long row_stride, in
     if (rows == 0) return 0;
     if (!logits || !s || !s->uniform || !tokens_out) return qdb_set_error("qdb_sample: null argument");
     const int es = type == QDB_TYPE_F32 ? 4 : 2;
-    if ((uintptr_t)logits % es) return qdb_set_error("qdb_sample: logits are not aligned to their type");
-    const QdbNamedPtr ps[] = {{logits, "logits"}, {s->temperature, "temperature"}, {s->top_k, "top_k"},
+    const QdbNamedPtr ps[] = {{logits, "logits", es}, {s->temperature, "temperature"}, {s->top_k, "top_k"},
                               {s->top_p, "top_p"}, {s->min_p, "min_p"}, {s->uniform, "uniform"},
                               {tokens_out, "tokens_out"}};
     if (qdb_check_device_ptrs("qdb_sample", ps, 7)) return -1;

@@ -188,6 +188,55 @@ def test_pool_refusals_and_lifetimes(pkg, synth, world):
     p2.close()
 
 
+def test_pool_in_a_freed_ones_place(pkg, synth, world):
+    """A captured step must not outlive its pool, though a new pool of another
+    page size may get the same memory."""
+    ws, model = world
+    emb = prompts(synth, ws, [70])[0]
+    one = model.session(128)
+    one.prefill(emb, 0)
+    _, _, want = one.forward(emb[3], 70, want_logits=True)
+    for page in (16, 64, 32, 128, 16):
+        pool = pkg.PagePool(model, 1024 // page, page)
+        s = [pool.session(), pool.session()]
+        pkg.prefill_batch(s, [emb[:40], emb], [0, 0])
+        for _ in range(3):  # (the second call captures, the third replays)
+            _, log = pkg.forward_batch(s, emb[[40, 3]], [40, 70], want_logits=True)
+            assert_logits_close(log[1], want, f"page {page}")
+        for x in s:
+            x.close()
+        pool.close()
+
+
+def test_sessions_without_rows_in_a_prefill(pkg, synth, world):
+    """No rows from any position: nothing happens to that session."""
+    ws, model = world
+    emb = prompts(synth, ws, [40])[0]
+    pool = pkg.PagePool(model, 16, 16)
+    a, b, c = pool.session(), pool.session(), pool.session()
+    pkg.prefill_batch([a, b, c], [emb[:0], emb, emb[:0]], [500, 0, 7])
+    assert (a.capacity, b.capacity, c.capacity) == (0, 48, 0)
+    one = model.session(64)
+    one.prefill(emb, 0)
+    _, _, want = one.forward(emb[3], 40, want_logits=True)
+    _, _, log = b.forward(emb[3], 40, want_logits=True)
+    assert_logits_close(log, want, "beside sessions without rows")
+
+
+def test_one_session_in_several_rows(pkg, synth, world):
+    """Two pieces of one session in one prefill, two of its positions in one step."""
+    ws, model = world
+    emb = prompts(synth, ws, [60])[0]
+    pool = pkg.PagePool(model, 16, 16)
+    s, one = pool.session(), model.session(64)
+    pkg.prefill_batch([s, s], [emb[:25], emb[25:50]], [0, 25])
+    one.prefill(emb[:50], 0)
+    _, log = pkg.forward_batch([s, s], emb[50:52], [50, 51], want_logits=True)
+    for i in range(2):
+        _, _, want = one.forward(emb[50 + i], 50 + i, want_logits=True)
+        assert_logits_close(log[i], want, f"row {i}")
+
+
 def test_injected_failures_leave_paged_calls_usable(pkg, synth, world, monkeypatch):
     ws, model = world
     pool = pkg.PagePool(model, 16, 16)

@@ -92,6 +92,18 @@ def test_bad_rows(pkg):
         kv(pkg, layout="dhn")
 
 
+@pytest.mark.parametrize("off", [1, 2, 3])
+def test_misaligned_arrays(pkg, off):
+    append, decode, prompt = ops(pkg)
+    for name in ("kv_lens", "tables", "err", "q_starts"):
+        for op in (append, prompt) if name == "q_starts" else (append, decode, prompt):
+            with pytest.raises(pkg.QdbError, match=f"{name} is not aligned"):
+                op(kv(pkg), batch(pkg, **{name: P + off}))
+    for name in ("temperature", "top_k", "top_p", "min_p", "uniform", "tokens"):
+        with pytest.raises(pkg.QdbError, match="is not aligned"):
+            pkg.sample(**{**dict(logits=P, rows=2, vocab=100, uniform=P, tokens=P), name: P + off})
+
+
 def test_null_structs(pkg):
     b, k = batch(pkg).c, kv(pkg).c
     assert pkg.lib.qdb_paged_decode(None, b, P, 0, 4, 0.0, P, 0, 1, None) == -1
