@@ -550,6 +550,78 @@ def test_side_stream_and_graph(pkg):
         check_attention(pool, q, out2, [1] * 3)
 
 
+def test_calls_on_two_streams_at_once(pkg):
+    """Decode and prompt calls that overlap on the GPU, each stream with its own workspace, give
+    what they give alone, bit for bit."""
+    sides = [torch.cuda.Stream() for _ in range(2)]
+    jobs = []
+    for i, side in enumerate(sides):
+        lens = [900 + 13 * i, 5, 3000, 64 + i]
+        q_lens = [300, 5, 700 + i, 1]
+        pool = Pool(pkg, lens, 2, 16 << i, ["f16", "bf16"][i], seed=20 + i)
+        q1, q2 = queries(4, 8, pool.dtype, seed=i), queries(sum(q_lens), 8, pool.dtype, seed=i)
+        jobs.append((side, pkg.PagedWorkspace(), pool, q1, torch.zeros_like(q1), q2, torch.zeros_like(q2), q_lens,
+                     starts_of(q_lens)))
+    torch.cuda.synchronize()
+
+    def go(job):
+        side, w, pool, q1, o1, q2, o2, _, st = job
+        s = side.cuda_stream
+        pkg.paged_decode(pool.kv(), pool.batch(), q1.data_ptr(), o1.data_ptr(), 8, w, stream=s)
+        pkg.paged_prompt(pool.kv(), pool.batch(rows=len(q2), starts=st), q2.data_ptr(), o2.data_ptr(), 8, stream=s)
+
+    alone = []
+    for job in jobs:
+        go(job)
+        torch.cuda.synchronize()
+        check_attention(job[2], job[3], job[4], [1] * 4)
+        check_attention(job[2], job[5], job[6], job[7])
+        alone.append((job[4].clone(), job[6].clone()))
+    for _ in range(30):
+        for job in jobs:
+            job[4].fill_(9), job[6].fill_(9)
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for job in jobs:
+                go(job)
+        torch.cuda.synchronize()
+        for job, (o1, o2) in zip(jobs, alone):
+            assert torch.equal(job[4], o1) and torch.equal(job[6], o2)
+
+
+def test_thousands_of_short_sequences(pkg, ws):
+    rng = np.random.default_rng(11)
+    n = 3000
+    lens = rng.integers(0, 40, n).tolist()
+    pool = Pool(pkg, lens, 2, 16, "f16", seed=12)
+    q = queries(n, 4, "f16")
+    check_attention(pool, q, run_decode(pkg, ws, pool, q), [1] * n)
+    q_lens = [int(rng.integers(0, m + 1)) for m in lens]
+    q = queries(sum(q_lens), 4, "f16")
+    check_attention(pool, q, run_prompt(pkg, pool, q, q_lens), q_lens)
+
+
+def test_rows_ahead_of_the_first_sequence(pkg):
+    """q_starts may begin above 0: the rows before belong to nobody and stay as they are."""
+    lens, q_lens, ahead = [300, 0, 40], [290, 0, 3], 37
+    pool = Pool(pkg, lens, 2, 16, "bf16", seed=8)
+    q = queries(ahead + sum(q_lens), 4, "bf16")
+    out = torch.full_like(q, 7.0)
+    st = starts_of(q_lens) + ahead
+    pkg.paged_prompt(pool.kv(), pool.batch(rows=len(q), starts=st), q.data_ptr(), out.data_ptr(), 4, stream=stream())
+    torch.cuda.synchronize()
+    assert (out[:ahead] == 7.0).all()
+    check_attention(pool, q[ahead:], out[ahead:], q_lens)
+    qkv = torch.randn(len(q), 8 * D, device="cuda")
+    new = torch.full_like(q, 7.0)
+    pkg.paged_append(pool.kv(), pool.batch(rows=len(q), starts=st), qkv.data_ptr(), new.data_ptr(), 4, stream=stream())
+    torch.cuda.synchronize()
+    assert (new[:ahead] == 7.0).all()
+    assert torch.equal(new[ahead:].reshape(-1, 4 * D), qkv[ahead:, :4 * D].to(torch.bfloat16))
+    assert torch.equal(pool.get(2, 40)[1][37:], qkv[-3:, 6 * D:].view(3, 2, D).to(torch.bfloat16))
+    assert pool.err.tolist() == [0, 0, 0, 0]
+
+
 def test_pool_offsets_beyond_32_bits(pkg, ws):
     """A pool of more than 2^32 elements: pages at its very end are the ones read and written."""
     hk, page = 8, 256
