@@ -25,6 +25,10 @@
 //                   when the maximum grows by more than 2^8, so numerator and
 //                   denominator always share one m
 //   P               rounded to the cache's type (the type of V's own rounding)
+// The roles' code together does not fit the instruction caches, and what runs
+// once per item is fetched anew each time: loops over it are kept short and not
+// unrolled, nothing is divided, non-finite values are dealt with after the
+// stores. (64 prompts of 404 positions took 152 us with 83 KB of code, 99 with 58.)
 // Keys behind a row's position count nothing, whatever the cache holds there:
 // scores are replaced by -inf, and in the tiles that some row sees only in part
 // the values behind the last visible key and non-finite values are cleared
@@ -96,11 +100,10 @@ __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint3
         "l"(b), "r"(kind), "n"(ACC ? 1 : 0)
         : "memory");
 }
-template <bool ACC>
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t kind) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t kind, uint32_t more) {
     asm volatile(
         "{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(d),
-        "r"(a), "l"(b), "r"(kind), "n"(ACC ? 1 : 0)
+        "r"(a), "l"(b), "r"(kind), "r"(more)
         : "memory");
 }
 __device__ __forceinline__ bool elect() {
@@ -171,32 +174,31 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
-// Bounded wait that also ends when another role has given up.
-__device__ __forceinline__ bool wait_on(PromptSmem &sm, uint32_t bar, unsigned parity, int *err) {
+// Bounded wait that also ends when another role has given up. (Short: it is
+// inlined at every wait. The error is recorded once, at the end.)
+__device__ __forceinline__ bool wait_on(PromptSmem &sm, uint32_t bar, unsigned parity) {
     if (bar_try(bar, parity)) return true;
-    const long long t0 = clock64();
-    while (!bar_try(bar, parity)) {
-        if (*reinterpret_cast<volatile int *>(&sm.abort)) return false;
-        if (clock64() - t0 > QDB_SPIN_LIMIT_CYCLES) {
-            set_error(err, QDB_ERR_BARRIER_TIMEOUT);
+    const unsigned t0 = (unsigned)clock();
+    while (!bar_try(bar, parity))
+        if (*reinterpret_cast<volatile int *>(&sm.abort) || (unsigned)clock() - t0 > (unsigned)QDB_SPIN_LIMIT_CYCLES) {
             *reinterpret_cast<volatile int *>(&sm.abort) = 1;
             return false;
         }
-    }
     return true;
 }
 
 // Blocks of bq rows: sequence b's begin at number q_starts[b] / bq + b, which
 // leaves room for every sequence's last, partly filled block (the numbers
 // behind it are empty). The blocks with the longest histories come first.
-__device__ Block find_block(const QdbPagedAttnArgs &a, int bq, int i, int lane) {
+__device__ Block find_block(const QdbPagedAttnArgs &a, int bq, unsigned inv_bq, int i, int lane) {
     Block k{0, 0, 0, 0, false};
     const int n = a.bt.n_seqs, step = a.bt.step ? *a.bt.step : 0;
     int lo = 0;
     if (a.bt.q_starts) {  // the last sequence that begins at or before i, 32 candidates at a time
+#pragma unroll 1
         for (int size = n; size > 1;) {
             const int d = (size + 31) / 32, mid = lo + lane * d;
-            const bool in = lane * d < size && max(a.bt.q_starts[mid], 0) / bq + mid <= i;
+            const bool in = lane * d < size && (int)__umulhi(max(a.bt.q_starts[mid], 0), inv_bq) + mid <= i;
             const int last = 31 - __clz(__ballot_sync(0xffffffffu, in) | 1u);
             size = min(d, size - last * d);
             lo += last * d;
@@ -208,7 +210,7 @@ __device__ Block find_block(const QdbPagedAttnArgs &a, int bq, int i, int lane) 
     const int len = paged_len(a.bt, lo, a.kv.page_shift, step);
     int first, last;
     paged_rows(a.bt, lo, first, last);
-    const int j = a.bt.q_starts ? i - (first / bq + lo) : 0, blocks = (last - first + bq - 1) / bq;
+    const int j = a.bt.q_starts ? i - ((int)__umulhi(first, inv_bq) + lo) : 0, blocks = __umulhi(last - first + bq - 1, inv_bq);
     if (j < 0 || j >= blocks) return k;
     const int at = (blocks - 1 - j) * bq;
     k.b = lo;
@@ -297,7 +299,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
     // Every role walks through the CTA's items on its own, as warp 10 announces
     // them, and keeps its own counts of the barriers' phases.
     bool ok = true;
-    auto wait = [&](uint32_t bar, unsigned parity) { return __all_sync(0xffffffffu, wait_on(sm, bar, parity, err)); };
+    auto wait = [&](uint32_t bar, unsigned parity) { return __all_sync(0xffffffffu, wait_on(sm, bar, parity)); };
     int item = 0;
     Block blk;
     int g = 0;
@@ -320,16 +322,17 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
     auto clear_v = [&](unsigned st, int half, int keys) {
         uint4 *v = reinterpret_cast<uint4 *>(sm.v[st] + half * PT_HALF);
         const int mine = keys * 8;  // 16 bytes of key e / 8 (the swizzle moves them within their row only)
-        for (int e = mine + lane; e < (int)(PT_HALF / 16); e += 32) v[e] = make_uint4(0u, 0u, 0u, 0u);
         uint32_t acc = 0;
-#pragma unroll 8
-        for (int e = lane; e < mine; e += 32) {
-            const uint4 w = v[e];
+#pragma unroll 4
+        for (int e = lane; e < (int)(PT_HALF / 16); e += 32) {
+            uint4 w = v[e];
+            if (e >= mine) v[e] = w = make_uint4(0u, 0u, 0u, 0u);
             acc |= T::zero_times(w.w, T::zero_times(w.z, T::zero_times(w.y, T::zero_times(w.x, 0))));
         }
         if (T::any_nonfinite(acc)) {
             *reinterpret_cast<volatile int *>(&sm.item[(item - 1) % PT_ITEMS].nonfinite) = 1;
             __threadfence_block();
+#pragma unroll 1
             for (int e = lane; e < mine; e += 32) {
                 const uint4 w = v[e];
                 v[e] = make_uint4(T::clear_nonfinite(w.x), T::clear_nonfinite(w.y), T::clear_nonfinite(w.z),
@@ -343,7 +346,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
     if (warp < 8) {
         // ------------------------------------------------ softmax of row tile x
         const int x = warp >> 2, r = t & 127;
-        const int i = r / G;  // position in the row tile
+        const unsigned inv_g = (65536u + G - 1) / G;  // n / G = n * inv_g >> 16 for n < 128
+        const int i = (int)((unsigned)r * inv_g >> 16);  // position in the row tile
         const uint32_t ts = tm + ((uint32_t)(32 * (warp & 3)) << 16), tp = ts + 128 + x * 64, to = ts + 256 + x * 128;
         const float c = a.scale * 1.4426950408889634f;
         constexpr float shift = T::code == QDB_TYPE_F16 ? 6.f : 0.f;  // keeps f16 weights down to 2^-30 of the largest
@@ -433,46 +437,65 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
             if (ok && nt > 0) ok = done_before(nt);
             if (!ok) break;
             if (nx > 0) {
+                if (nt == 0) {  // nothing to see for any row
+                    uint32_t zero[32];
+#pragma unroll
+                    for (int e = 0; e < 32; e++) zero[e] = 0u;
+#pragma unroll 1
+                    for (int k = 0; k < 128; k += 32) tm_st32(to + k, zero);
+                    tm_st_wait();
+                }
                 const float scale_o = l > 0.f ? 1.0f / l : (isnan(l) ? l : 0.f);
                 const bool fix = *reinterpret_cast<const volatile int *>(nonfinite) != 0;  // (written before the products)
-                // a thread stores its own row, 64 dims at a time (passing rows through shared
-                // memory for full 128-byte stores took as long)
                 for (int part = 0; part < (PAIR ? 2 : 1); part++) {  // (hi, then lo of a bf16 pair)
                     auto word = [&](uint32_t y, uint32_t z) {
                         const float u = __uint_as_float(y), v = __uint_as_float(z);
                         return PAIR ? QdbBf16::plain(pair_part(u, part), pair_part(v, part)) : T::plain(u, v);
                     };
 #pragma unroll 1
-                    for (int k = 0; k < 128; k += 64) {
-                        uint32_t o[64];
-                        if (nt > 0) {
-                            tm_ld64(to + k, o);
-                        } else {
+                    for (int k = 0; k < 128; k += 32) {
+                        uint32_t o[32];
+                        tm_ld32(to + k, o);
 #pragma unroll
-                            for (int e = 0; e < 64; e++) o[e] = 0u;
-                        }
+                        for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * scale_o);
+                        // (two lanes exchange pieces: each store writes whole 32-byte sectors)
+                        const bool up = lane & 1;
+                        const int rr0 = r & ~1, i0 = (int)((unsigned)rr0 * inv_g >> 16), i1 = (int)((unsigned)(rr0 + 1) * inv_g >> 16);
+                        uint16_t *dst = (part ? a.lo : a.out) + (size_t)g * G * QDB_HD + k + (lane & 1) * 8;
+                        uint16_t *d0 = dst + (size_t)(sh.row0 + x * QP + i0) * a.out_stride + (rr0 - i0 * G) * QDB_HD;
+                        uint16_t *d1 = dst + (size_t)(sh.row0 + x * QP + i1) * a.out_stride + (rr0 + 1 - i1 * G) * QDB_HD;
+                        const bool r0 = i0 < nx && i0 < QP, r1 = i1 < nx && i1 < QP;
 #pragma unroll
-                        for (int e = 0; e < 64; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * scale_o);
-                        if (fix && real)  // non-finite values were left out of the products: add those this row sees
-                            for (int key = sh.special * PT_N; key <= pos; key++) {
-                                const int page = paged_page(a.kv, a.bt, sh.b, key >> a.kv.page_shift);
-                                if (page < 0) continue;
-                                const uint16_t *v = a.kv.v + page * a.kv.page_stride + g * a.kv.head_stride +
-                                                    (key & ((1 << a.kv.page_shift) - 1)) * a.kv.pos_stride + k;
+                        for (int e = 0; e < 32; e += 16) {
+                            uint32_t lo[4], hi[4];
 #pragma unroll
-                                for (int e = 0; e < 64; e++) {
-                                    const float y = T::lo(v[e]);
-                                    if (!isfinite(y)) o[e] = __float_as_uint(__uint_as_float(o[e]) + y);
-                                }
+                            for (int z = 0; z < 4; z++) {
+                                const uint32_t p = word(o[e + 2 * z], o[e + 2 * z + 1]), q = word(o[e + 8 + 2 * z], o[e + 9 + 2 * z]);
+                                const uint32_t got = __shfl_xor_sync(0xffffffffu, up ? p : q, 1);
+                                lo[z] = up ? got : p;
+                                hi[z] = up ? q : got;
                             }
-                        if (real) {
-                            uint16_t *dst = (part ? a.lo : a.out) + (size_t)(sh.row0 + x * QP + i) * a.out_stride +
-                                            ((size_t)g * G + r - i * G) * QDB_HD + k;
-#pragma unroll
-                            for (int e = 0; e < 64; e += 8)
-                                *reinterpret_cast<uint4 *>(dst + e) =
-                                    make_uint4(word(o[e], o[e + 1]), word(o[e + 2], o[e + 3]), word(o[e + 4], o[e + 5]),
-                                               word(o[e + 6], o[e + 7]));
+                            if (r0) *reinterpret_cast<uint4 *>(d0 + e) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                            if (r1) *reinterpret_cast<uint4 *>(d1 + e) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                        }
+                    }
+                }
+                if (fix) {  // non-finite values were left out of the products: add those each row sees
+                    __syncwarp();
+                    if (real) {
+                        uint16_t *dst = a.out + (size_t)(sh.row0 + x * QP + i) * a.out_stride + ((size_t)g * G + r - i * G) * QDB_HD;
+#pragma unroll 1
+                        for (int key = sh.special * PT_N; key <= pos; key++) {
+                            const int page = paged_page(a.kv, a.bt, sh.b, key >> a.kv.page_shift);
+                            if (page < 0) continue;
+                            const uint16_t *v = a.kv.v + page * a.kv.page_stride + g * a.kv.head_stride +
+                                                (key & ((1 << a.kv.page_shift) - 1)) * a.kv.pos_stride;
+#pragma unroll 1
+                            for (int e = 0; e < QDB_HD; e++) {
+                                const float y = T::lo(v[e]);
+                                if (isfinite(y)) continue;
+                                dst[e] = PAIR ? QdbBf16::plain1(QdbBf16::lo(dst[e]) + y) : T::plain1(T::lo(dst[e]) + y);
+                            }
                         }
                     }
                 }
@@ -508,15 +531,15 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
             const uint64_t v = v_desc + st * tile;
             const uint32_t d = tmu + 256 + x * 128, p = tmu + 128 + x * 64;
             if (leader) {
-                if (more) mma_ts<true>(d, p, v, op_kind<T>(true));
-                else mma_ts<false>(d, p, v, op_kind<T>(true));
+                mma_ts(d, p, v, op_kind<T>(true), more);
 #pragma unroll
-                for (int e = 1; e < 8; e++) mma_ts<true>(d, p + e * 8, v + e * (2048 >> 4), op_kind<T>(true));
+                for (int e = 1; e < 8; e++) mma_ts(d, p + e * 8, v + e * (2048 >> 4), op_kind<T>(true), 1);
                 commit(smem_u32(&sm.o_done[x]));
             }
             __syncwarp();
         };
-        unsigned n_tile = 0, n_part = 0, n_q = 0, n_s = 0, n_p0 = 0, n_p1 = 0;
+        unsigned st = 0, phase = 0;  // ring stage of the next tile, how often the ring has gone round (mod 2)
+        unsigned n_part = 0, n_q = 0, n_s = 0, n_p0 = 0, n_p1 = 0;
         while (next_item()) {
             const Shape sh(blk, g, QP);
             const int T0 = __shfl_sync(0xffffffffu, sh.t0, 0), T1 = __shfl_sync(0xffffffffu, sh.t1, 0), TT = max(T0, T1);
@@ -525,14 +548,14 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
             if (TT == 0) continue;
             if (scores_warp) ok = wait(smem_u32(&sm.q_full), n_q++ & 1);
             // row tiles 0 and 1 in turn, tile after tile
-            for (int j = 0; j < TT && ok; j++, n_tile++) {
-                const unsigned st = n_tile % (scores_warp ? PT_KS : PT_VS), use = n_tile / (scores_warp ? PT_KS : PT_VS);
-                ok = wait(smem_u32(scores_warp ? &sm.k_full[st] : &sm.v_full[st]), use & 1);
+            for (int j = 0; j < TT && ok; j++) {
+                ok = wait(smem_u32(scores_warp ? &sm.k_full[st] : &sm.v_full[st]), phase);
                 if (!scores_warp && ok && j >= part) {  // warp 11 clears the other half
                     clear_v(st, 0, min(sh.end - j * PT_N, PT_N));
                     ok = wait(smem_u32(&sm.v_clean[n_part % PT_PART]), (n_part / PT_PART) & 1);
                     n_part++;
                 }
+#pragma unroll 1
                 for (int x = 0; x < 2 && ok; x++) {
                     if (j >= (x ? T1 : T0)) continue;
                     if (scores_warp) {  // (the scores before have been read)
@@ -548,6 +571,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                 }
                 if (ok && leader) commit(smem_u32(scores_warp ? &sm.k_empty[st] : &sm.v_empty[st]));
                 __syncwarp();
+                if (++st == (scores_warp ? PT_KS : PT_VS)) st = 0, phase ^= 1;
             }
             if (!ok) break;
             if (scores_warp && leader) commit(smem_u32(&sm.q_empty));
@@ -561,16 +585,17 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
     } else {
         // ------------------------------------------------ copies: warp 10 Q and K (and the items), warp 11 V
         const bool is_v = warp == 11, leader = elect();
-        const int rows = min(1 << a.kv.page_shift, PT_N), pieces = PT_N / rows, S = is_v ? PT_VS : PT_KS;
+        const int rsh = min(a.kv.page_shift, 7), rows = 1 << rsh, pieces = PT_N >> rsh, S = is_v ? PT_VS : PT_KS;
         unsigned long long *full = is_v ? sm.v_full : sm.k_full, *empty = is_v ? sm.v_empty : sm.k_empty;
         const uint32_t ring = smem_u32(is_v ? sm.v[0] : sm.k[0]);
         const CUtensorMap *map = is_v ? &mv : &mk;
-        unsigned n_tile = 0, n_q = 0, n_part = 0;
+        unsigned n_tile = 0, n_q = 0, n_part = 0, st = 0, phase = 0;
         // The CTA's items: its own number, then those of CTAs that have not been
         // launched yet, taken from the launch queue until none is left. It asks for
         // the next one two tiles before this one's end: at once, a CTA with a heavy
         // item would keep a second one from those that will be free before it.
         int number = blockIdx.x;
+        const unsigned inv_bq = 0xffffffffu / (2 * QP) + 1;  // n / bq = n * inv_bq >> 32 for n < 2^23, bq <= 256
         unsigned asked = 0, answered = 0;
         auto ask = [&] {
             if (leader) {
@@ -585,8 +610,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
             asked++;
         };
         auto answer = [&] {  // the number taken, or -1: none is left
-            ok = wait(smem_u32(&sm.stolen_bar), answered++ & 1);
+            ok = wait(smem_u32(&sm.stolen_bar), answered & 1);
             if (!ok) return -1;
+            answered++;
             const volatile uint64_t *w = sm.stolen;
             const uint64_t lo = w[0], hi = w[1];
             uint32_t got, x = 0;
@@ -609,15 +635,18 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                     if (!ok) return false;
                 }
                 Block k{0, 0, 0, 0, false};
+                int kh = 0;
                 if (number >= 0) {
-                    k = find_block(a, 2 * QP, number / Hkv, lane);
+                    const int blk_no = number / Hkv;
+                    k = find_block(a, 2 * QP, inv_bq, blk_no, lane);
+                    kh = number - blk_no * Hkv;
                     if (!k.any) continue;
                 }
                 const int s = item % PT_ITEMS;
                 if (item >= PT_ITEMS) ok = wait(smem_u32(&sm.item_empty[s]), ((item / PT_ITEMS) & 1) ^ 1);
                 if (!ok) return false;
                 blk = k;
-                g = number >= 0 ? number % Hkv : 0;
+                g = kh;
                 if (lane == 0) {
                     sm.item[s] = Item{k, g, 0};
                     bar_arrive(smem_u32(&sm.item_full[s]));
@@ -640,17 +669,21 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                 if (is_v) item_done();
                 continue;
             }
-            int page = look_up(0);
+            int page = -1;
             const int end = __shfl_sync(0xffffffffu, sh.end, 0), head = __shfl_sync(0xffffffffu, g, 0);
-            for (int j = 0; j < sh.tiles; j++) {
-                const int n = min(pieces, (end - j * PT_N + rows - 1) / rows), slot = (j * PT_N) & ((1 << a.kv.page_shift) - 1);
+            for (int j = -1; j < sh.tiles; j++) {
                 const int after = j + 1 < sh.tiles ? look_up(j + 1) : -1;  // (not waited for before it is needed)
-                const unsigned st = n_tile % S;
-                if (n_tile >= (unsigned)S) ok = wait(smem_u32(&empty[st]), ((n_tile / S) & 1) ^ 1);
+                if (j < 0) {
+                    page = after;
+                    continue;
+                }
+                const int n = min(pieces, (end - j * PT_N + rows - 1) >> rsh), slot = (j * PT_N) & ((1 << a.kv.page_shift) - 1);
+                if (n_tile >= (unsigned)S) ok = wait(smem_u32(&empty[st]), phase ^ 1);
                 if (!ok) break;
                 // pieces one after the other, all operands the same in every lane
                 const uint32_t dst = ring + st * PT_TILE, bar = smem_u32(&full[st]);
                 if (leader) bar_expect(bar, (uint32_t)n * rows * 256u);
+#pragma unroll 1
                 for (int p = 0; p < n; p++) {
                     const int pg = __shfl_sync(0xffffffffu, page, p);
                     if (leader) {
@@ -660,6 +693,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                 }
                 __syncwarp();
                 n_tile++;
+                if (++st == (unsigned)S) st = 0, phase ^= 1;
                 page = after;
                 if (is_v) continue;
                 if (j == 0) {  // Q, once the item before has no more use for its rows
@@ -687,9 +721,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                 // ones, no more than the ring holds, so none waits for another's clearing)
                 for (int j = sh.special; j < sh.tiles; j++, n_part++) {
                     const unsigned k = n_tile - sh.tiles + j;
-                    ok = wait(smem_u32(&full[k % S]), (k / S) & 1);
+                    ok = wait(smem_u32(&sm.v_full[k % PT_VS]), (k / PT_VS) & 1);
                     if (!ok) break;
-                    clear_v(k % S, 1, min(end - j * PT_N, PT_N));
+                    clear_v(k % PT_VS, 1, min(end - j * PT_N, PT_N));
                     if (leader) bar_arrive(smem_u32(&sm.v_clean[n_part % PT_PART]));
                 }
                 if (!ok) break;
@@ -697,15 +731,27 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
             }
         }
         if (!ok) {  // given up: what is in flight lands first
-            if (asked > answered) bar_wait(smem_u32(&sm.stolen_bar), answered & 1, err);
-            if (n_q) bar_wait(smem_u32(&sm.q_full), (n_q - 1) & 1, err);
-            for (unsigned k = n_tile > (unsigned)S ? n_tile - S : 0; k < n_tile; k++)
-                bar_wait(smem_u32(&full[k % S]), (k / S) & 1, err);
+            const int ring_tiles = min(n_tile, (unsigned)S);
+#pragma unroll 1
+            for (int k = -2; k < ring_tiles; k++) {
+                uint32_t bar = smem_u32(&sm.stolen_bar);
+                unsigned parity = answered & 1;
+                if (k == -2 && asked == answered) continue;
+                if (k == -1) {
+                    if (!n_q) continue;
+                    bar = smem_u32(&sm.q_full), parity = (n_q - 1) & 1;
+                } else if (k >= 0) {  // (the ring's tiles, the newest first)
+                    if (st-- == 0) st = S - 1, phase ^= 1;
+                    bar = smem_u32(&full[st]), parity = phase;
+                }
+                bar_wait(bar, parity, err);
+            }
         }
         __syncwarp();
     }
     tc_before();
     __syncthreads();
+    if (t == 0 && sm.abort) set_error(err, QDB_ERR_BARRIER_TIMEOUT);
     if (warp == 8) {
         tc_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "r"(512) : "memory");
