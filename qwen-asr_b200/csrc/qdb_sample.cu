@@ -11,10 +11,11 @@
 // -inf.
 //
 // Sums are 64-bit integers: w is rounded to a multiple of 2^-45 (a token more
-// than 31.5 T below the maximum is never drawn), so a sum over up to 2^18 tokens is exact, independent
-// of the order of the atomics, and a border between two tokens is off by at
-// most 2^-46 of the largest weight per token summed. (uniform = 0 asks for the
-// first kept token of any weight above zero: there every such token counts 1.)
+// than 31.5 T below the maximum is never drawn), so a sum over up to 2^18 tokens
+// is exact, independent of the order of the atomics, and a border between two
+// tokens is off by at most 2^-46 of the largest weight per token summed.
+// (uniform = 0 asks for the first kept token of any weight above zero: there
+// every such token counts 1.)
 //
 // A row is read from HBM once: a cluster of up to 8 CTAs (as many as leave each
 // at least 16K tokens) keeps it in shared memory as order-preserving integers.
@@ -29,6 +30,15 @@
 // finds the last token that stays; every CTA then draws from its own tokens.
 // Bins of more than 2048 (many equal logits) are cut by a radix selection. All
 // ways take the same integer weights, so they give the same token.
+//
+// Measured, 151936 f32 logits a row: one row with top_k 50 and top_p 0.95 14 us
+// (5 us greedy, 41 us top_p alone), 64 rows of mixed parameters 51 us, 18 rows of
+// top_k 50 19 us. Reading the logits would take 0.1 and 6 us: what bounds it is
+// the chain of cluster barriers (1000 clocks each) and passes for one row, and the
+// instructions per token for many (45 in the pass that weighs and counts all
+// tokens: a weight to 2^-45 takes about 11 64-bit operations). A first version,
+// one CTA per row and the logits read again in every pass, took 609 and
+// 3176 us.
 #include <cooperative_groups.h>
 #include <math.h>
 #include <stdio.h>
@@ -87,6 +97,7 @@ struct alignas(16) SampleSmem {
     union {
         struct {
             unsigned n[BINS], f[BINS];  // tokens; their places within the bin, in 1 / 4096, added up
+            // (also the scratch of a sorting list, which goes on into f)
         } hist;
         u64 val[LIST];
     };
@@ -107,6 +118,7 @@ struct alignas(16) SampleSmem {
     unsigned offset;
     u64 cut;         // the last token that stays
     int lo, hi;      // first CTA
+    uint32_t ends[2];
     Plan plan;
     Pick pick;
 };
@@ -129,10 +141,12 @@ __device__ __forceinline__ X block_scan(X v, X *buf, int lane, int warp, X *all)
 }
 
 // n2 (a power of two, at least 64) values, all different but for zeros, in
-// descending order. Up to 128 by counting the larger ones of each; more by a
-// bitonic network, whose steps over distances up to 32 stay within 64 values of
-// one warp.
-__device__ void sort_down(u64 *x, int n2, int t) {
+// descending order. Up to 128 by counting the larger ones of each; more by
+// buckets of equal width, in which each value counts the larger ones (583 values:
+// 5300 clocks, the bitonic network 15900); where a bucket has too many for that
+// (equal logits), by a bitonic network, whose steps over distances up to 32 stay
+// within 64 values of one warp. scratch: BINS + 2 words.
+__device__ void sort_down(u64 *x, int n2, unsigned *scratch, unsigned *scan, int t) {
     __syncthreads();
     if (n2 <= 128) {
         const u64 mine = t < n2 ? x[t] : 0;
@@ -150,6 +164,64 @@ __device__ void sort_down(u64 *x, int n2, int t) {
         __syncthreads();
         return;
     }
+    constexpr int MINE = LIST / ST, FULL = 32;
+    static_assert(BINS == ST * MINE, "a thread has as many buckets as values");
+    u64 v[MINE];
+    unsigned hi = 0, lo = 0xffffffffu;
+#pragma unroll
+    for (int e = 0; e < MINE; e++) {
+        v[e] = t + e * ST < n2 ? x[t + e * ST] : 0;
+        if (v[e]) hi = max(hi, (unsigned)(v[e] >> 32)), lo = min(lo, (unsigned)(v[e] >> 32));
+        scratch[t + e * ST] = 0;
+    }
+    unsigned *ends = scratch + BINS;
+    if (t == 0) ends[0] = 0, ends[1] = 0xffffffffu;
+    __syncthreads();
+    hi = __reduce_max_sync(0xffffffffu, hi);
+    lo = __reduce_min_sync(0xffffffffu, lo);
+    if ((t & 31) == 0) {
+        atomicMax(ends, hi);
+        atomicMin(ends + 1, lo);
+    }
+    __syncthreads();
+    hi = ends[0];
+    const float per = (float)BINS / ((float)(hi - ends[1]) + 1.f);  // (monotone: rounding moves no value past another)
+    int bucket[MINE];
+    unsigned slot[MINE];
+    bool full = false;
+#pragma unroll
+    for (int e = 0; e < MINE; e++) {
+        bucket[e] = min(BINS - 1, (int)((float)(hi - (unsigned)(v[e] >> 32)) * per));
+        slot[e] = v[e] ? atomicAdd(scratch + bucket[e], 1u) : 0;
+        full |= slot[e] >= FULL;
+    }
+    if (!__syncthreads_or(full)) {
+        const uint4 c = reinterpret_cast<const uint4 *>(scratch)[t];
+        unsigned m;
+        const unsigned first = block_scan<unsigned>(c.x + c.y + c.z + c.w, scan, t & 31, t >> 5, &m);
+        reinterpret_cast<uint4 *>(scratch)[t] = make_uint4(first, first + c.x, first + c.x + c.y, first + c.x + c.y + c.z);
+        if (t == 0) scratch[BINS] = m;
+        __syncthreads();
+        unsigned at[MINE];
+#pragma unroll
+        for (int e = 0; e < MINE; e++)
+            if (v[e]) x[at[e] = scratch[bucket[e]] + slot[e]] = v[e];
+        for (int i = m + t; i < n2; i += ST) x[i] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < MINE; e++) {
+            if (!v[e]) continue;
+            const unsigned b0 = scratch[bucket[e]], b1 = scratch[bucket[e] + 1];
+            at[e] = b0;
+            for (unsigned i = b0; i < b1; i++) at[e] += x[i] > v[e];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < MINE; e++)
+            if (v[e]) x[at[e]] = v[e];
+        __syncthreads();
+        return;
+    }
     for (int k = 2; k <= n2; k <<= 1)
         for (int j = k >> 1; j > 0; j >>= 1) {
             for (int p = t; p < n2 / 2; p += ST) {
@@ -164,25 +236,63 @@ __device__ void sort_down(u64 *x, int n2, int t) {
     __syncthreads();
 }
 
+// What a row's parameters ask for: 0 the largest logit, 1 the threads' maxima
+// and a short list, 2 passes over all its tokens. C: CTAs of its cluster.
+struct Asked {
+    float T, top_p, min_p;
+    int top_k;
+    __device__ __forceinline__ Asked(const QdbSampleArgs &a, int row)
+        : T(a.temperature ? a.temperature[row] : 1.f), top_p(a.top_p ? a.top_p[row] : 1.f),
+          min_p(a.min_p ? a.min_p[row] : 0.f), top_k(a.top_k ? a.top_k[row] : 0) {}
+    __device__ __forceinline__ bool greedy() const { return !(T > 0.f) || top_p <= 0.f || min_p > 1.f || top_k == 1; }
+    __device__ __forceinline__ int work(int C) const { return greedy() ? 0 : top_k > 0 && top_k <= C * ST / 4 ? 1 : 2; }
+};
+
+// Where not all clusters run at once, those that start first take the rows with
+// the most work: the cluster's row, ordered so within its 128 rows (64 rows of
+// mixed parameters: 67 us in the rows' own order, 56 so).
+__device__ __forceinline__ int heavy_first(const QdbSampleArgs &a, int at, int C, int lane) {
+    const int first = at & ~127;
+    int nth = at - first, work[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const int row = first + e * 32 + lane;
+        work[e] = row < a.rows ? Asked(a, row).work(C) : -1;
+    }
+    for (int w = 2; w >= 0; w--)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const unsigned b = __ballot_sync(0xffffffffu, work[e] == w);
+            if (nth < __popc(b)) {
+                const unsigned hit = __ballot_sync(0xffffffffu, (b >> lane & 1) && __popc(b & ((1u << lane) - 1)) == nth);
+                return first + e * 32 + __ffs(hit) - 1;
+            }
+            nth -= __popc(b);
+        }
+    return at;  // (not reached)
+}
+
 template <int TYPE>
-__global__ void __launch_bounds__(ST, 2) sample_kernel(const QdbSampleArgs a, int slice) {
+__global__ void __launch_bounds__(ST, 2) sample_kernel(const QdbSampleArgs a, int slice, bool ordered) {
     extern __shared__ __align__(16) unsigned char smem_raw[];
     SampleSmem &sm = *reinterpret_cast<SampleSmem *>(smem_raw);
     uint32_t *keys = reinterpret_cast<uint32_t *>(smem_raw + sizeof(SampleSmem));
     cg::cluster_group cl = cg::this_cluster();
-    const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank(), row = blockIdx.x / C;
+    const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank();
+    int row = blockIdx.x / C;
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5, V = a.vocab;
     const int base = min(V, rank * slice), n = min(V, base + slice) - base;  // this CTA's tokens
     SampleSmem *lead = cl.map_shared_rank(&sm, 0);
     for (int i = t; i < BINS; i += ST) sm.hist.n[i] = 0, sm.hist.f[i] = 0;
-    if (t == 0) sm.weight = 0, sm.count = 0;
+    if (t == 0) sm.weight = 0, sm.count = 0, sm.total[0] = 0;
     if (t < 16) sm.exp2_16[t] = exp2(45.0 + t / 16.0);
     cl.barrier_arrive();  // (waited for before the first access to another CTA's memory)
     pdl_enter();
+    if (ordered) row = heavy_first(a, row, C, lane);
     const size_t out_at = (a.step ? (size_t)*a.step * a.rows : 0) + row;
-    const float T = a.temperature ? a.temperature[row] : 1.f;
-    const int top_k = a.top_k ? a.top_k[row] : 0;
-    const float top_p = a.top_p ? a.top_p[row] : 1.f, min_p = a.min_p ? a.min_p[row] : 0.f;
+    const Asked ask(a, row);
+    const float T = ask.T, top_p = ask.top_p, min_p = ask.min_p;
+    const int top_k = ask.top_k;
     const float u = a.uniform[out_at];
 
     // ---- 1. the row into shared memory; its maximum
@@ -261,7 +371,7 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const QdbSampleArgs a, in
         best = sm.best[r] > best ? sm.best[r] : best;
         low = min(low, sm.low[r]);
     }
-    if (best == 0 || !(T > 0.f) || top_p <= 0.f || min_p > 1.f || top_k == 1) {
+    if (best == 0 || ask.greedy()) {
         if (rank == 0 && t == 0) a.tokens[out_at] = best ? (int)(0xffffffffu - (uint32_t)best) : -1;
         return;
     }
@@ -312,27 +422,20 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const QdbSampleArgs a, in
         for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
         return v;
     };
-    // Tokens that `take` wants to the first CTA's list (in any order); a
-    // barrier of the cluster has to follow. Each CTA collects in its own list.
-    auto gather = [&](uint32_t from, auto take) {
+    // Tokens to the first CTA's list (in any order): each CTA collects in its own
+    // list, then sends it; a barrier of the cluster has to follow.
+    auto open_list = [&] {
         if (rank) {
             __syncthreads();
             if (t == 0) sm.count = 0;
             __syncthreads();
         }
-        if (bk >= from)  // (else this thread has no key from there on)
-        each4([&](int i, const uint32_t *k) {
-            bool yes[4];
-#pragma unroll
-            for (int e = 0; e < 4; e++) yes[e] = take(k[e], i + e);
-            if (!(yes[0] | yes[1] | yes[2] | yes[3])) return;
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-                if (yes[e]) {
-                    const unsigned at = atomicAdd(&sm.count, 1u);
-                    if (at < LIST) sm.list[at] = token_of(k[e], i + e);
-                }
-        });
+    };
+    auto push = [&](uint32_t k, int i) {
+        const unsigned at = atomicAdd(&sm.count, 1u);
+        if (at < LIST) sm.list[at] = token_of(k, i);
+    };
+    auto send_list = [&] {
         if (rank) {
             __syncthreads();
             if (t == 0) sm.offset = atomicAdd(&lead->count, sm.count);
@@ -342,13 +445,27 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const QdbSampleArgs a, in
                 if (at + i < LIST) lead->list[at + i] = sm.list[i];
         }
     };
+    auto gather = [&](uint32_t from, auto take) {  // those that `take` wants, none below `from`
+        open_list();
+        if (bk >= from)  // (else this thread has no key from there on)
+            each4([&](int i, const uint32_t *k) {
+                bool yes[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) yes[e] = take(k[e], i + e);
+                if (!(yes[0] | yes[1] | yes[2] | yes[3])) return;
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    if (yes[e]) push(k[e], i + e);
+            });
+        send_list();
+    };
     // First CTA: sorts the list; returns its length.
     auto sort_list = [&](int *n2) {
         const int m = min((int)sm.count, LIST);
         *n2 = 64;
         while (*n2 < m) *n2 <<= 1;
         for (int i = m + t; i < *n2; i += ST) sm.list[i] = 0;
-        sort_down(sm.list, *n2, t);
+        sort_down(sm.list, *n2, sm.hist.n, reinterpret_cast<unsigned *>(sm.scan), t);  // (the histogram has been used)
         return m;
     };
     constexpr int PT = BINS / ST;  // bins, or list entries, of a thread
@@ -432,7 +549,7 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const QdbSampleArgs a, in
             before += w[e];
             if (i < n2) sm.val[i] = x;
         }
-        sort_down(sm.val, n2, t);
+        sort_down(sm.val, n2, reinterpret_cast<unsigned *>(sm.list), reinterpret_cast<unsigned *>(sm.scan), t);
         mine = 0;
 #pragma unroll
         for (int e = 0; e < PT; e++) {
@@ -452,25 +569,42 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const QdbSampleArgs a, in
     };
     unsigned cn = 0, all_n;  // first CTA: tokens and (in f32) weight ahead of this thread's bins
     float cw = 0.f, all_w;
-    // First CTA: adds up the cluster's histograms. A bin's weight is taken as its
-    // tokens times the weight at their mean place: off by less than 2^-14, since
-    // weights within a bin differ by at most a factor of 1.016.
+    // Adds up the cluster's histograms with their places: each CTA its share of the
+    // bins, into the first CTA's.
+    auto merge = [&] {
+        if (C == 1) return;
+        const int share = BINS / C;
+        for (int i = t; i < 2 * share; i += ST) {
+            const int bin = rank * share + (i < share ? i : i - share);
+            unsigned sum = 0;
+#pragma unroll
+            for (int r = 0; r < SC; r++)
+                if (r < C) {
+                    const SampleSmem *o = cl.map_shared_rank(&sm, r);
+                    sum += i < share ? o->hist.n[bin] : o->hist.f[bin];
+                }
+            if (i < share) lead->hist.n[bin] = sum;
+            else lead->hist.f[bin] = sum;
+        }
+        cl.sync();
+    };
+    // First CTA: counts (and weights, of merged histograms) ahead of each thread's
+    // bins. A bin's weight is taken as its tokens times the weight at their mean
+    // place: off by less than 2^-14, since weights within a bin differ by at most a
+    // factor of 1.016.
     float bin_w[PT];
     auto collect = [&](bool weights) {
         static_assert(PT == 4, "a thread's bins are one vector");
         uint4 bn = reinterpret_cast<const uint4 *>(sm.hist.n)[t], bf = reinterpret_cast<const uint4 *>(sm.hist.f)[t];
+        if (!weights) {
 #pragma unroll
-        for (int r = 1; r < SC; r++)
-            if (r < C) {
-                const SampleSmem *o = cl.map_shared_rank(&sm, r);
-                const uint4 y = reinterpret_cast<const uint4 *>(o->hist.n)[t];
-                bn.x += y.x, bn.y += y.y, bn.z += y.z, bn.w += y.w;
-                if (weights) {
-                    const uint4 z = reinterpret_cast<const uint4 *>(o->hist.f)[t];
-                    bf.x += z.x, bf.y += z.y, bf.z += z.z, bf.w += z.w;
+            for (int r = 1; r < SC; r++)
+                if (r < C) {
+                    const uint4 y = reinterpret_cast<const uint4 *>(cl.map_shared_rank(&sm, r)->hist.n)[t];
+                    bn.x += y.x, bn.y += y.y, bn.z += y.z, bn.w += y.w;
                 }
-            }
-        reinterpret_cast<uint4 *>(sm.hist.n)[t] = bn;
+            reinterpret_cast<uint4 *>(sm.hist.n)[t] = bn;
+        }
         cn = block_scan<unsigned>(bn.x + bn.y + bn.z + bn.w, reinterpret_cast<unsigned *>(sm.scan), lane, warp, &all_n);
         if (weights) {
             const unsigned cnt[PT] = {bn.x, bn.y, bn.z, bn.w}, pl[PT] = {bf.x, bf.y, bf.z, bf.w};
@@ -554,6 +688,7 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const QdbSampleArgs a, in
             if (lane == 0) atomicAdd(&lead->weight, sum);
         }
         cl.sync();
+        if (need_w) merge();
         // First CTA: bins lo .. hi that hold the end of the top_p for a given
         // total weight. The f32 weights are taken to be off by up to 2^-11 (what was
         // found is checked).
@@ -636,13 +771,20 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const QdbSampleArgs a, in
             }
         }
         if (way == P_BINS) {  // the end of the top_p
-            // keys from .. to - 1 are in bins lo .. hi
-            const uint32_t from = bin_start(sm.plan.hi), to = sm.plan.lo ? bin_start(sm.plan.lo - 1) : kmax + 1;
-            const u64 w = range_sum([&](uint32_t k, int i) { return (k >= to) & (token_of(k, i) >= cut); });
-            if (t == 0 && rank == 0) sm.total[0] = 0;
-            cl.sync();
+            // keys from .. to - 1 are in bins lo .. hi (the ends found side by side)
+            const uint32_t end = warp & 1 ? (sm.plan.lo ? bin_start(sm.plan.lo - 1) : kmax + 1) : bin_start(sm.plan.hi);
+            if (lane == 0 && warp < 2) sm.ends[warp] = end;
+            open_list();
+            __syncthreads();
+            const uint32_t from = sm.ends[0], to = sm.ends[1];
+            // one pass: the weight of the tokens above those bins, and the bins' tokens
+            const u64 w = range_sum([&](uint32_t k, int i) {
+                const bool in = (k >= from) & (token_of(k, i) >= cut);
+                if (in & (k < to)) push(k, i);
+                return in & (k >= to);
+            });
             if (lane == 0) atomicAdd(&lead->total[0], w);
-            gather(from, [&](uint32_t k, int i) { return (k >= from) & (k < to) & (token_of(k, i) >= cut); });
+            send_list();
             cl.sync();
             if (rank == 0) {
                 int n2;
@@ -675,10 +817,8 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const QdbSampleArgs a, in
             way = sm.plan.way;
             if (way == P_BINS) {
                 cut = sm.cut;
-                if (min_cut <= (u64)to << 32) {  // the sum goes on with the last bins' tokens
-                    range = w + range_sum([&](uint32_t k, int i) {
-                        return (k < to) & (token_of(k, i) >= cut) & (token_of(k, i) >= min_cut);
-                    });
+                if (!min_cut) {  // the sum goes on with the last bins' tokens
+                    range = w + range_sum([&](uint32_t k, int i) { return (k < to) & (token_of(k, i) >= cut); });
                     have_range = true;
                 }
             }
@@ -840,6 +980,11 @@ cudaError_t launch(const QdbSampleArgs &a, cudaStream_t st) {
     const size_t smem = sizeof(SampleSmem) + (size_t)slice * 4;
     cudaError_t e = cudaFuncSetAttribute(sample_kernel<TYPE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
+    int dev = 0, sms = 0;
+    if ((e = cudaGetDevice(&dev)) != cudaSuccess ||
+        (e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess)
+        return e;
+    const bool ordered = (a.temperature || a.top_k || a.top_p || a.min_p) && (long long)a.rows * C > 2 * sms;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(a.rows * C);
     cfg.blockDim = dim3(ST);
@@ -853,7 +998,7 @@ cudaError_t launch(const QdbSampleArgs &a, cudaStream_t st) {
     attr[1].val.programmaticStreamSerializationAllowed = QDB_PDL;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, sample_kernel<TYPE>, a, slice);
+    return cudaLaunchKernelEx(&cfg, sample_kernel<TYPE>, a, slice, ordered);
 }
 
 }  // namespace

@@ -138,6 +138,35 @@ def test_row_stride_and_many_rows(pkg):
     assert run(pkg, y, u, row_stride=777, dtype="bf16", **kw) == want(y[:, :772], u, **kw)
 
 
+@pytest.mark.parametrize("vocab,rows", [(40, 700), (20000, 333), (151936, 131)])
+def test_rows_of_all_kinds_beside_each_other(pkg, vocab, rows):
+    """More rows than run at once: which row is taken when depends on its parameters, its token not."""
+    rng = np.random.default_rng(rows)
+    x = logits(rows, vocab, seed=rows)
+    u = rng.random(rows).astype(np.float32).tolist()
+    kw = dict(temp=rng.choice([0.0, 0.4, 1.0, float("nan")], rows).tolist(),
+              k=rng.choice([0, 1, 5, 400, 1500], rows).tolist(), p=rng.choice([1.0, 0.9, 0.5, 0.0], rows).tolist(),
+              floor=rng.choice([0.0, 0.02, 2.0], rows).tolist())
+    got = run(pkg, x, u, **kw)
+    assert got == want(x, u, **kw)
+    for one in ("temp", "k", "p", "floor"):
+        assert run(pkg, x, u, **{one: kw[one]}) == want(x, u, **{one: kw[one]})
+
+
+@pytest.mark.parametrize("equal", [1, 5, 31, 32, 33, 100, 1000])
+def test_lists_with_groups_of_equal_logits(pkg, equal):
+    """Lists of 129 to 2048 tokens whose logits come in groups."""
+    rng = np.random.default_rng(equal)
+    vocab, rows = 30000, 10
+    level = rng.permutation(vocab) // equal
+    x = torch.tensor(-0.004 * equal * level, device="cuda").float().repeat(rows, 1)
+    x[1::2] += torch.tensor(rng.normal(size=(rows // 2, 1)), device="cuda").float()
+    u = rng.random(rows).astype(np.float32).tolist()
+    for kw in (dict(k=[129] * rows), dict(k=[700] * rows, p=[0.8] * rows), dict(k=[1900] * rows), dict(p=[0.99] * rows),
+               dict(p=[0.6] * rows, temp=[3.0] * rows), dict(p=[0.9] * rows, floor=[0.01] * rows)):
+        assert run(pkg, x, u, **kw) == want(x, u, **kw)
+
+
 def test_frequencies(pkg):
     """Evenly spaced random numbers give each token its share of the draws, to within one draw."""
     x = torch.tensor([[0.0, 1.0, 2.0, -1.0]], device="cuda").repeat(4096, 1)
