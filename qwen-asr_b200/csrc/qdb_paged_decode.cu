@@ -19,9 +19,9 @@
 // does not depend on timing.
 //
 // Measured (L2 cold): 256 ragged sequences of 1 to 1500 tokens, 16 heads on 8
-// key heads, bf16, 148 us, and 8 of 24000 to 32768, 32 heads on 4, 84 us: 89 %
-// and 82 % of the copy bandwidth for their K and V bytes. 64 sequences of 404
-// to 660, f16, 32 us against 21 for the bytes; one of 404 9.7 us against 0.3:
+// key heads, bf16, 147 us, and 8 of 24000 to 32768, 32 heads on 4, 83 us: 89 %
+// and 83 % of the copy bandwidth for their K and V bytes. 64 sequences of 404
+// to 660, f16, 32 us against 21 for the bytes; one of 404 9.1 us against 0.3:
 // the fixed chain of launch, lengths, page numbers, first tiles and the join
 // over CTAs. A first version with one CTA per pair, plain loads and scalar
 // products took 11.5 ms, 734 us, 344 us and 91 us for the four.
@@ -39,7 +39,7 @@ constexpr int TILE = 16;          // keys per tile (a page holds whole tiles)
 constexpr int TILE_B = 4096;      // bytes of a tile's K (or V)
 constexpr int MAX_G = 16;         // query heads per key head
 // Tiles of a CTA, on average, below which a pair is not cut further. 404 keys
-// of 8 key heads: 9.5 us at 4, 9.9 at 8, 11.6 at 16; 4000 keys: 11.8 us at 4 to
+// of 8 key heads: 9.5 us at 4, 9.9 at 8, 11.6 at 16 (before later steps); 4000 keys: 11.8 us at 4 to
 // 16, 13.8 at 32.
 constexpr int MIN_TILES = 4;
 constexpr float P_SHIFT = 8.0f;   // P is scaled by 2^8: f16 keeps weights down to 2^-32 of the largest
@@ -120,6 +120,10 @@ struct Joined {
 template <typename ML, typename Row>
 __device__ __forceinline__ Joined join(int n, int lane, ML ml, Row row) {
     Joined j;
+    constexpr int AHEAD = 8;  // parts on their way while the weights are computed
+    float4 first[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; i++) first[i] = i < n ? row(i) : make_float4(0.f, 0.f, 0.f, 0.f);
     j.m = -INFINITY;
     for (int i = lane; i < n; i += 32) j.m = fmaxf(j.m, ml(i).x);
     j.m = warp_max(j.m);
@@ -134,15 +138,19 @@ __device__ __forceinline__ Joined join(int n, int lane, ML ml, Row row) {
         }
         j.l += warp_sum(l);
         const int k = min(32, n - i0);
-#pragma unroll 8
-        for (int i = 0; i < k; i++) {
-            const float4 x = row(i0 + i);
+        auto add = [&](const float4 &x, int i) {
             const float f = __shfl_sync(0xffffffffu, w, i);
             j.o[0] = fmaf(x.x, f, j.o[0]);
             j.o[1] = fmaf(x.y, f, j.o[1]);
             j.o[2] = fmaf(x.z, f, j.o[2]);
             j.o[3] = fmaf(x.w, f, j.o[3]);
-        }
+        };
+        if (i0 == 0)
+#pragma unroll
+            for (int i = 0; i < AHEAD; i++)
+                if (i < k) add(first[i], i);
+#pragma unroll 8
+        for (int i = i0 ? 0 : AHEAD; i < k; i++) add(row(i0 + i), i);
     }
     return j;
 }
@@ -535,15 +543,15 @@ __global__ void __launch_bounds__(DW * 32, 1)
     if (!split) return;
     // ---- pairs over several CTAs (at most the first and the last of this one):
     // the CTA whose part arrives last joins them
-    __threadfence();
     __syncthreads();
     if (t <= DW && sm.grp[t].some && sm.grp[t].c0 != sm.grp[t].c1) {
         const Group gr = sm.grp[t];
-        if (atomicAdd(&ws.cnt[gr.c0], 1u) == (unsigned)(gr.c1 - gr.c0)) {
+        unsigned before;  // (releases this CTA's parts, acquires the others')
+        asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(ws.cnt + gr.c0) : "memory");
+        if (before == (unsigned)(gr.c1 - gr.c0)) {
             sm.todo[t ? 1 : 0] = t;
             ws.cnt[gr.c0] = 0;  // nobody else comes
         }
-        __threadfence();
     }
     __syncthreads();
     item = 0;
