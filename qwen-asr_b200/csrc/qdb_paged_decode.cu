@@ -19,9 +19,9 @@
 // does not depend on timing.
 //
 // Measured (L2 cold): 256 ragged sequences of 1 to 1500 tokens, 16 heads on 8
-// key heads, bf16, 147 us, and 8 of 24000 to 32768, 32 heads on 4, 83 us: 89 %
-// and 83 % of the copy bandwidth for their K and V bytes. 64 sequences of 404
-// to 660, f16, 32 us against 21 for the bytes; one of 404 9.1 us against 0.3:
+// key heads, bf16, 144 us, and 8 of 24000 to 32768, 32 heads on 4, 80 us: 92 %
+// and 86 % of the copy bandwidth for their K and V bytes. 64 sequences of 404
+// to 660, f16, 31 us against 21 for the bytes; one of 404 8.1 us against 0.3:
 // the fixed chain of launch, lengths, page numbers, first tiles and the join
 // over CTAs. A first version, one warp per (row, query head) with scalar
 // products, took 734 us for the 256, 11.5 ms, 344 and 91 us.
@@ -111,46 +111,60 @@ struct Cursor {
     int b, g, tile, nt, len;
 };
 
-// Joins parts 0 .. n-1 of one head: ml(i) = (m, l), row(i) = this lane's 4 dims.
-// The weights 2^(m_i - max) are computed one part per lane, then every lane
-// adds up its dims in the order of the parts.
+// Joins parts 0 .. n-1 of one head, in their order: ml(i) = (m, l), row(i) = this
+// lane's 4 dims; the weights are 2^(m_i - max).
 struct Joined {
     float m, l, o[4];
+    __device__ __forceinline__ void add(const float4 &x, float w) {
+        o[0] = fmaf(x.x, w, o[0]);
+        o[1] = fmaf(x.y, w, o[1]);
+        o[2] = fmaf(x.z, w, o[2]);
+        o[3] = fmaf(x.w, w, o[3]);
+    }
 };
+__device__ __forceinline__ float part_weight(float m, float top) { return m == top ? 1.f : exp2f(m - top); }  // (also of -inf)
+// Up to FEW parts: all loads at once, every lane weighs them all (64 sequences 32.4
+// -> 30.6 us, one 9.1 -> 8.1 against reductions over the warp).
+constexpr int FEW = DW;  // (the parts within a CTA)
+template <typename ML, typename Row>
+__device__ __forceinline__ Joined join_few(int n, ML ml, Row row) {
+    float2 x[FEW];
+    float4 r[FEW];
+#pragma unroll
+    for (int i = 0; i < FEW; i++) {
+        x[i] = i < n ? ml(i) : make_float2(-INFINITY, 0.f);
+        r[i] = i < n ? row(i) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    Joined j{x[0].x, 0.f, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+    for (int i = 1; i < FEW; i++) j.m = fmaxf(j.m, x[i].x);
+#pragma unroll
+    for (int i = 0; i < FEW; i++) {
+        if (i >= n) break;
+        const float w = part_weight(x[i].x, j.m);
+        j.l += x[i].y * w;
+        j.add(r[i], w);
+    }
+    return j;
+}
+// Any number: the weights are computed one part per lane.
 template <typename ML, typename Row>
 __device__ __forceinline__ Joined join(int n, int lane, ML ml, Row row) {
-    Joined j;
-    constexpr int AHEAD = 8;  // parts on their way while the weights are computed
-    float4 first[AHEAD];
-#pragma unroll
-    for (int i = 0; i < AHEAD; i++) first[i] = i < n ? row(i) : make_float4(0.f, 0.f, 0.f, 0.f);
-    j.m = -INFINITY;
+    if (n <= FEW) return join_few(n, ml, row);
+    Joined j{-INFINITY, 0.f, {0.f, 0.f, 0.f, 0.f}};
     for (int i = lane; i < n; i += 32) j.m = fmaxf(j.m, ml(i).x);
     j.m = warp_max(j.m);
-    j.l = 0.f;
-    j.o[0] = j.o[1] = j.o[2] = j.o[3] = 0.f;
     for (int i0 = 0; i0 < n; i0 += 32) {
         float w = 0.f, l = 0.f;
         if (i0 + lane < n) {
             const float2 x = ml(i0 + lane);
-            w = x.x == j.m ? 1.f : exp2f(x.x - j.m);  // (also where both are -inf)
+            w = part_weight(x.x, j.m);
             l = x.y * w;
         }
         j.l += warp_sum(l);
         const int k = min(32, n - i0);
-        auto add = [&](const float4 &x, int i) {
-            const float f = __shfl_sync(0xffffffffu, w, i);
-            j.o[0] = fmaf(x.x, f, j.o[0]);
-            j.o[1] = fmaf(x.y, f, j.o[1]);
-            j.o[2] = fmaf(x.z, f, j.o[2]);
-            j.o[3] = fmaf(x.w, f, j.o[3]);
-        };
-        if (i0 == 0)
-#pragma unroll
-            for (int i = 0; i < AHEAD; i++)
-                if (i < k) add(first[i], i);
 #pragma unroll 8
-        for (int i = i0 ? 0 : AHEAD; i < k; i++) add(row(i0 + i), i);
+        for (int i = 0; i < k; i++) j.add(row(i0 + i), __shfl_sync(0xffffffffu, w, i));
     }
     return j;
 }
@@ -523,8 +537,8 @@ __global__ void __launch_bounds__(DW * 32, 1)
         for (int h = 0; h < G; h++, item++) {
             if (item % DW != warp) continue;
             const Group gr = sm.grp[k];
-            const Joined j = join(
-                gr.w1 - gr.w0 + 1, lane,
+            const Joined j = join_few(
+                gr.w1 - gr.w0 + 1,
                 [&](int i) { return sm.ml[gr.w0 + i][i == 0 && k ? 1 : 0][h]; },
                 [&](int i) {
                     const float *src = i == 0 && k ? reinterpret_cast<const float *>(&sm.ring[gr.w0][0][0][0])
