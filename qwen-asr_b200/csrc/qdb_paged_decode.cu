@@ -19,8 +19,8 @@
 // does not depend on timing.
 //
 // Measured (L2 cold): 256 ragged sequences of 1 to 1500 tokens, 16 heads on 8
-// key heads, bf16, 144 us, and 8 of 24000 to 32768, 32 heads on 4, 80 us: 92 %
-// and 86 % of the copy bandwidth for their K and V bytes. 64 sequences of 404
+// key heads, bf16, 144 us, and 8 of 24000 to 32768, 32 heads on 4, 78 us: 91 %
+// and 88 % of the copy bandwidth for their K and V bytes. 64 sequences of 404
 // to 660, f16, 31 us against 21 for the bytes; one of 404 8.1 us against 0.3:
 // the fixed chain of launch, lengths, page numbers, first tiles and the join
 // over CTAs. A first version, one warp per (row, query head) with scalar
@@ -42,6 +42,9 @@ constexpr int MAX_G = 16;         // query heads per key head
 // of 8 key heads: 9.5 us at 4, 9.9 at 8, 11.6 at 16 (before later steps); 4000 keys: 11.8 us at 4 to
 // 16, 13.8 at 32.
 constexpr int MIN_TILES = 4;
+// Tiles of a CTA from which the pairs' borders do not matter: 8 sequences of 24000
+// to 32768 with 4 key heads 80.1 us on 128 CTAs, 78.2 on all 148.
+constexpr int MANY_TILES = 128;
 constexpr float P_SHIFT = 8.0f;   // P is scaled by 2^8: f16 keeps weights down to 2^-32 of the largest
 
 // Ring stages per warp: what shared memory leaves beside one partial per warp.
@@ -242,18 +245,19 @@ __global__ void __launch_bounds__(DW * 32, 1)
     sm.find.before[t] = before;
     total *= Hkv;
     if (total == 0) return;
-    // CTAs that take part: all of them where there are more pairs than CTAs;
-    // else a whole number per pair (equal lengths then need no join beyond the
-    // pair's own), each with at least MIN_TILES tiles on average, and no more than
-    // sqrt(16 tiles / G), at which the joining CTA reads as many bytes of parts as
-    // each CTA has read of K and V (one history of 32000 with 16 heads on one key
-    // head: 39.2 us with all 148 CTAs, 27.2 with these 44); never so many that a
-    // warp would have no tile (a range is empty only where one CTA does it all)
+    // CTAs that take part: all of them where there are more pairs than CTAs, or
+    // MANY_TILES for each; else a whole number per pair (equal lengths then need no
+    // join beyond the pair's own), each with at least MIN_TILES tiles on average, and
+    // no more than sqrt(16 tiles / G), at which the joining CTA reads as many bytes
+    // of parts as each CTA has read of K and V (one history of 32000 with 16 heads
+    // on one key head: 39.2 us with all 148 CTAs, 27.2 with these 44); never so many
+    // that a warp would have no tile (a range is empty only where one CTA does it all)
     int ctas = ws.ctas;
     if ((long long)n * Hkv <= ctas) {
         const int np = n * Hkv;
         const int most = (int)sqrtf(16.f * (float)(total / np) / (float)G);
-        ctas = np * max(1, min(min(ctas / np, most), total / (np * MIN_TILES)));
+        if (ctas / np > most || total / ctas < MANY_TILES)
+            ctas = np * max(1, min(min(ctas / np, most), total / (np * MIN_TILES)));
     }
     ctas = min(ctas, max(total / DW, 1));
     if ((int)blockIdx.x >= ctas) return;
