@@ -642,11 +642,21 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const QdbSampleArgs a, in
     // the threads' largest keys is a lower bound of the top_k-th key, and few
     // tokens lie above it.
     if (k_on && !first && top_k <= C * ST / 4) {
-        if (bk >= least) atomicAdd(&sm.hist.n[bin_of(bk)], 1u);
+        // (four bins taken together: a quarter of the reads from the other CTAs, and a
+        // list that is hardly longer)
+        static_assert(PT == 4, "a thread has four bins");
+        if (bk >= least) atomicAdd(&sm.hist.n[bin_of(bk) / PT], 1u);
         cl.sync();
         if (rank == 0) {
-            collect(false);
-            k_bin();
+            unsigned here = sm.hist.n[t];
+#pragma unroll
+            for (int r = 1; r < SC; r++)
+                if (r < C) here += cl.map_shared_rank(&sm, r)->hist.n[t];
+            if (t == 0) sm.hi = BINS - 1;
+            unsigned all;
+            const unsigned before = block_scan<unsigned>(here, reinterpret_cast<unsigned *>(sm.scan), lane, warp, &all);
+            if (before < (unsigned)top_k && (unsigned)top_k <= before + here) sm.hi = t * PT + PT - 1;
+            __syncthreads();
             tell(ALL_LISTED, 0, sm.hi);
         }
         cl.sync();
