@@ -29,6 +29,11 @@
 // once per item is fetched anew each time: loops over it are kept short and not
 // unrolled, nothing is divided, non-finite values are dealt with after the
 // stores. (64 prompts of 404 positions took 152 us with 83 KB of code, 99 with 58.)
+// Measured, 16 heads on 8 key heads: 16384 positions bf16 813 us in short bursts
+// (1.35 PFLOP/s), 950 run on and on, where power sets the clock; 3721 positions
+// 55 us; 64 pieces of 30 to 130 rows behind up to 400 cached positions 38 us; one
+// prompt of 404 13 us, most of it the chain of look-ups, copies and four tiles. A
+// first version on the CUDA cores took 182 ms for the 16384, 1.7 ms for the pieces.
 // Keys behind a row's position count nothing, whatever the cache holds there:
 // scores are replaced by -inf, and in the tiles that some row sees only in part
 // the values behind the last visible key and non-finite values are cleared

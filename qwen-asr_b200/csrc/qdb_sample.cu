@@ -32,7 +32,7 @@
 // ways take the same integer weights, so they give the same token.
 //
 // Measured, 151936 f32 logits a row: one row with top_k 50 and top_p 0.95 12.6 us
-// (4.7 us greedy, 40 us top_p alone), 64 rows of mixed parameters 50 us, 18 rows of
+// (4.7 us greedy, 40 us top_p alone), 64 rows of mixed parameters 49 us, 18 rows of
 // top_k 50 17 us. Reading the logits would take 0.1 and 6 us: what bounds it is
 // the chain of cluster barriers (1000 clocks each) and passes for one row, and the
 // instructions per token for many (45 in the pass that weighs and counts all
@@ -406,6 +406,9 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const QdbSampleArgs a, in
         return (u64)__double_as_longlong(w + 4503599627370496.0) & ((1ull << 52) - 1);
     };
     auto weight = [&](uint32_t k) { return whole_weight(real_weight(k)); };
+    // The same as a double: a thread's up to 64 tokens add up to an exact integer
+    // below 2^52, without the 64-bit additions' instructions.
+    auto whole = [&](double w) { return (w + 4503599627370496.0) - 4503599627370496.0; };
     // Calls f(i, k) for this CTA's tokens i .. i + 3 with keys k[4], whose
     // arithmetic then overlaps (0 behind the end).
     auto each4 = [&](auto f) {
@@ -510,7 +513,7 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const QdbSampleArgs a, in
     // The weight of this warp's tokens that `take` wants (weights are computed
     // only where some lane has one).
     auto range_sum = [&](auto take) {
-        u64 sum = 0;
+        double sum = 0.0;
         for (int i = i0 + lane * 4; i - lane * 4 < i1; i += 128) {
             uint4 x = make_uint4(0u, 0u, 0u, 0u);
             if (i < i1) x = *reinterpret_cast<const uint4 *>(keys + i);
@@ -521,11 +524,11 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const QdbSampleArgs a, in
             if (!__any_sync(0xffffffffu, yes[0] | yes[1] | yes[2] | yes[3])) continue;
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                const u64 w = weight(k[e]);
-                sum += yes[e] ? w : 0;
+                const double w = whole(real_weight(k[e]));
+                sum += yes[e] ? w : 0.0;
             }
         }
-        return warp_total(sum);
+        return warp_total((u64)sum);
     };
     u64 range = 0;           // of the tokens that stay, if known
     bool have_range = false;
@@ -684,7 +687,7 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const QdbSampleArgs a, in
     }
     if ((k_on || p_on) && !first) {
         const bool need_w = p_on && (!k_on || top_k > LIST);
-        u64 sum = 0;
+        double mine = 0.0;
         each4([&](int, const uint32_t *k) {
             int b[4];
 #pragma unroll
@@ -694,7 +697,7 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const QdbSampleArgs a, in
             }
             if (need_w && !k_on)
 #pragma unroll
-                for (int e = 0; e < 4; e++) sum += weight(k[e]);
+                for (int e = 0; e < 4; e++) mine += whole(real_weight(k[e]));
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 if (b[e] < 0) continue;
@@ -703,7 +706,7 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const QdbSampleArgs a, in
             }
         });
         if (p_on && !k_on) {
-            sum = warp_total(sum);
+            const u64 sum = warp_total((u64)mine);
             if (lane == 0) atomicAdd(&lead->weight, sum);
         }
         cl.sync();
