@@ -197,6 +197,15 @@ def test_decode_random_batches(pkg, ws):
         check_attention(pool, q, run_decode(pkg, ws, pool, q), [1] * n, what=f"batch {it}")
 
 
+@pytest.mark.parametrize("dtype,heads,kv_heads", [("f16", 8, 4), ("bf16", 32, 4), ("bf16", 16, 1)])
+def test_decode_long_histories(pkg, ws, dtype, heads, kv_heads):
+    """Long enough that shares of the tile list begin and end anywhere in a history."""
+    lens = [60000, 50001, 0, 44443] if kv_heads > 1 else [200000, 131073, 17]
+    pool = Pool(pkg, lens, kv_heads, 64, dtype, seed=14)
+    q = queries(len(lens), heads, dtype)
+    check_attention(pool, q, run_decode(pkg, ws, pool, q), [1] * len(lens))
+
+
 def test_decode_large_scores(pkg, ws):
     """One key far above the rest, and late: the running maximum moves by hundreds."""
     for dtype in ("f16", "bf16"):
