@@ -434,7 +434,8 @@ typedef struct {
  * values into the cache and the queries to q_out [rows, heads * 128] in the
  * cache's type. f16 stores saturate at +-65504. row_stride / q_stride: elements
  * between rows (0 = contiguous), multiples of 16 bytes. A row at a negative
- * position (more rows than kv_lens) is left out. Up to 16 query heads per key
+ * position (more rows than kv_lens), or behind the page table or the rotation
+ * table (recorded in err), is left out: nothing of it is written. Up to 16 query heads per key
  * head. A position must not occur twice in one call, and the rows, q_out and the
  * cache must not overlap. */
 int qdb_paged_append(const qdb_paged_kv *kv, const qdb_paged_batch *batch, const void *qkv, int src_type,

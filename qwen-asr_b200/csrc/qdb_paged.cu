@@ -97,10 +97,12 @@ __global__ void __launch_bounds__(AP_THREADS, AP_CTAS) append_kernel(const QdbAp
     int first, last;
     paged_rows(a.bt, b, first, last);
     if (row < first || row >= last) return;
-    const int len = paged_len(a.bt, b, a.kv.page_shift, a.bt.step ? *a.bt.step : 0);
-    const int pos = len - (last - row);
-    if (pos < 0) return;  // the sequence is shorter than its rows
-    // a row that cannot be rotated is left out whole
+    const long long at64 = (long long)a.bt.lens[b] + (a.bt.step ? *a.bt.step : 0) - (last - row);
+    if (at64 < 0) return;  // the sequence is shorter than its rows
+    // a row that has no place in the page table, or cannot be rotated, is left out whole
+    const bool held = at64 >> a.kv.page_shift < a.bt.table_stride;
+    if (!check_or_record(held, a.bt.err, QDB_CHECK_TABLE, b, at64)) return;
+    const int pos = (int)at64;
     if (a.rope && !check_or_record(pos < a.rope_len, a.bt.err, QDB_CHECK_ROPE, b, pos)) return;
     float4 cs[4];  // (cos, sin) of two pairs each
     if (a.rope && s0 < Hq + Hkv) {

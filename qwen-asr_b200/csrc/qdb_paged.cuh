@@ -16,7 +16,7 @@
 // Which check refused an access (err[1] of the caller's error words).
 enum {
     QDB_CHECK_PAGE = 1,    // page id outside the pool: err[2] = sequence, err[3] = page id
-    QDB_CHECK_TABLE = 2,   // position behind the table's end: err[2] = sequence, err[3] = position
+    QDB_CHECK_TABLE = 2,   // behind the table's end: err[2] = sequence, err[3] = length (append: position)
     QDB_CHECK_ROPE = 3,    // position behind the rotation table: err[2] = sequence, err[3] = position
     QDB_CHECK_STARTS = 4,  // row range outside [0, rows] or backwards: err[2] = sequence, err[3] = its end
 };
@@ -94,7 +94,7 @@ struct QdbBf16 {
     }
 };
 
-// Length of sequence b: never negative, never behind its page table.
+// Length of sequence b for reading: never negative, never behind its page table.
 __device__ __forceinline__ int paged_len(const QdbPagedBatch &bt, int b, int page_shift, int step) {
     long long n = (long long)bt.lens[b] + step;
     const long long most = (long long)bt.table_stride << page_shift;

@@ -1,0 +1,60 @@
+"""GPU: the paged-cache operators and paged sessions at the ends of what they hold."""
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from test_gpu_paged import D, T, Pool, append64, half_step, rope_table, starts_of, stream  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------- rows behind the page table
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("layout", ["hnd", "nhd"])
+@pytest.mark.parametrize("rope", [True, False])
+@pytest.mark.parametrize("over,new", [(1, 1), (1, 9), (40, 9), (40, 60), (1 << 20, 3)])
+def test_append_leaves_out_rows_behind_the_table(pkg, dtype, layout, rope, over, new):
+    """A sequence that has outgrown its page table by `over` positions: of its `new` newest rows
+    those the table still holds go where they belong, the others nowhere (neither to an earlier
+    position nor, where the table is padded with a valid id, to another sequence's page), and the
+    first of them is recorded. The sequences beside it are served."""
+    page, heads, hk = 16, 4, 2
+    full = 3 * page
+    pool = Pool(pkg, [full, 30, full], hk, page, dtype, layout, seed=over)
+    tab = torch.tensor(pool.tab[:, :3], device="cuda")
+    tab[1, 2] = tab[0, 0]  # padded with a valid id
+    tab = tab.contiguous()
+    lens = [full + over, full + over, full]
+    q_lens = [new, 1, 1]
+    starts = starts_of(q_lens)
+    lens_dev = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    rows = sum(q_lens)
+    qkv = torch.randn(rows, (heads + 2 * hk) * D, generator=torch.Generator("cuda").manual_seed(3), device="cuda")
+    q = torch.full((rows, heads, D), 7.0, device="cuda", dtype=T[dtype])
+    table = rope_table((1 << 20) + 64 if over > 40 else 256) if rope else None
+    batch = pkg.PagedBatch(3, rows, lens_dev.data_ptr(), tab.data_ptr(), 3, q_starts=starts.data_ptr(),
+                           err=pool.err.data_ptr())
+    k0, v0 = pool.k.clone(), pool.v.clone()
+    pkg.paged_append(pool.kv(), batch, qkv.data_ptr(), q.data_ptr(), heads, rope=table.data_ptr() if rope else 0,
+                     rope_len=len(table) if rope else 0, stream=stream())
+    torch.cuda.synchronize()
+    pos = np.concatenate([np.arange(n - m, n) for m, n in zip(q_lens, lens)])
+    inside = torch.tensor(pos < full, device="cuda")
+    at = torch.tensor(np.minimum(pos, full - 1), device="cuda")
+    wq, wk, wv, size = append64(qkv, heads, hk, at, table, None, None, 1e-6)
+    u = half_step(dtype)
+    near = lambda got, want, sz: ((got.double() - want).abs() <= u * want.abs() + 2.0 ** -20 * sz + 2.0 ** -25).all()  # noqa: E731
+    assert (q[~inside] == 7.0).all()
+    assert near(q[inside], wq[inside], size[inside][:, :heads])
+    for r in torch.nonzero(inside).flatten().tolist():
+        b = int(np.searchsorted(np.cumsum(q_lens), r, side="right"))
+        pg, sl = int(pool.tab[b, pos[r] // page]), int(pos[r] % page)
+        for c, c0, w in ((pool.k, k0, wk), (pool.v, v0, wv)):
+            got = c[pg, :, sl] if layout == "hnd" else c[pg, sl]
+            assert near(got, w[r], size[r, heads:] if c is pool.k else 0.0)
+            got.copy_(c0[pg, :, sl] if layout == "hnd" else c0[pg, sl])  # (put back: the rest is untouched)
+    for c, c0 in ((pool.k, k0), (pool.v, v0)):
+        assert torch.equal(c.view(torch.int16), c0.view(torch.int16))
+    err = pool.err.tolist()
+    assert err[:2] == [3, 2] and err[2] in (0, 1) and err[3] in pos[pos >= full]
