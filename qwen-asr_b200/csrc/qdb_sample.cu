@@ -53,6 +53,7 @@ typedef unsigned long long u64;
 constexpr int ST = 512, SW = ST / 32;       // threads and warps per CTA
 constexpr int SC = 8;                       // CTAs per cluster, at most
 constexpr int BINS = 2048, LIST = 2048;     // histogram bins; tokens the first CTA takes
+constexpr int SLICE = QDB_SAMPLE_MAX_VOCAB / SC;  // tokens per CTA, at most
 constexpr double S_ONE = 35184372088832.0;  // 2^45
 constexpr float S_REACH = 31.5f;            // exp(-31.5) = 2^-45.4: what lies further down is left out
 
@@ -1000,7 +1001,11 @@ cudaError_t launch(const QdbSampleArgs &a, cudaStream_t st) {
     while (C < SC && a.vocab > C * 16384) C <<= 1;
     const int slice = ((a.vocab + C - 1) / C + 31) & ~31;
     const size_t smem = sizeof(SampleSmem) + (size_t)slice * 4;
-    cudaError_t e = cudaFuncSetAttribute(sample_kernel<TYPE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    // the limit belongs to the kernel, not to this call: always the largest, so that
+    // calls of other sizes from other threads find it high enough
+    constexpr size_t most = sizeof(SampleSmem) + (size_t)SLICE * 4;
+    static_assert(SLICE >= 16384 && SLICE % 32 == 0 && most <= 227 * 1024, "a CTA's tokens fit its shared memory");
+    cudaError_t e = cudaFuncSetAttribute(sample_kernel<TYPE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
     if (e != cudaSuccess) return e;
     int dev = 0, sms = 0;
     if ((e = cudaGetDevice(&dev)) != cudaSuccess ||
