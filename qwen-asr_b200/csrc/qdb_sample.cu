@@ -767,7 +767,8 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const QdbSampleArgs a, in
             if (rank == 0) {
                 int n2;
                 const int m = sort_list(&n2);
-                const u64 last = sm.list[min(m, top_k - (int)sm.pick.above) - 1];
+                // (an empty bin: the tokens that weigh are fewer than top_k, so all of them stay)
+                const u64 last = m ? sm.list[min(m, top_k - (int)sm.pick.above) - 1] : (u64)least << 32;
                 if (t < C) cl.map_shared_rank(&sm, t)->cut = last;
                 __syncthreads();
                 if (t == 0) sm.count = 0;

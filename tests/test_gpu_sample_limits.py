@@ -5,7 +5,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from test_gpu_sample import logits, want  # noqa: E402
+from test_gpu_sample import logits, run, want  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -44,3 +44,20 @@ def test_threads_with_different_vocabularies(pkg):
     assert not failed
     for got, ref in out.values():
         assert got == ref
+
+
+@pytest.mark.parametrize("vocab", [16000, 60000, 151936])
+@pytest.mark.parametrize("allowed", [2049, 5000, 10000])
+@pytest.mark.parametrize("mask", [-1e9, -1e4, float("-inf")])
+def test_top_k_above_the_tokens_that_weigh(pkg, vocab, allowed, mask):
+    """Thousands of tokens allowed, the rest masked with finite values far below, top_k between
+    the allowed ones and the vocabulary: all allowed tokens stay."""
+    rows = 8
+    x = torch.full((rows, vocab), mask, device="cuda")
+    at = torch.randperm(vocab, generator=torch.Generator("cuda").manual_seed(allowed), device="cuda")[:allowed]
+    x[:, at] = logits(rows, allowed, seed=vocab, spread=1.0)
+    u = [0.0, 0.1, 0.3, 0.5, 0.7, 0.9, 0.99, 0.9999]
+    for k in (allowed - 1, allowed, allowed + 1, (allowed + vocab) // 2, vocab - 1):
+        for kw in (dict(), dict(p=[0.9] * rows), dict(floor=[0.05] * rows), dict(p=[0.7] * rows, temp=[0.6] * rows)):
+            kw = dict(kw, k=[k] * rows)
+            assert run(pkg, x, u, **kw) == want(x, u, **kw), (k, kw)
