@@ -610,12 +610,16 @@ extern "C" void qdb_session_free(qdb_session *s) {
 
 extern "C" int qdb_session_capacity(const qdb_session *s) { return s ? s->cap : 0; }
 
+// Positions of a session, at most (capacities double in ints).
+static constexpr int MAX_POSITIONS = 1 << 30;
+
 // Grows the cache (doubling, like kv_cache_grow, qwen_asr_decoder.c:133-160)
 // and keeps the first `cap` positions of every (layer, kv head) block.
 extern "C" int qdb_session_reserve(qdb_session *s, int positions) {
     if (!s) return fail("null session");
     if (!s->m) return fail("session's model has been freed");
     if (positions <= s->cap) return 0;
+    if (positions > MAX_POSITIONS) return fail("%d positions exceed the limit of 2^30", positions);
     qdb_model *m = s->m;
     if (set_dev(m)) return -1;
     if (qdb_pool *p = s->pool) {  // more pages, nothing moves
@@ -789,9 +793,10 @@ static int launch_step(qdb_model *m, QdbStepArgs &a) {
     return 0;
 }
 
-static int prep_pos(qdb_session *s, int last_pos) {
-    if (qdb_session_reserve(s, last_pos + 1)) return -1;
-    return ensure_rope(s->m, last_pos + 1);
+static int prep_pos(qdb_session *s, long long last_pos) {
+    if (last_pos >= MAX_POSITIONS) return fail("position %lld is behind the limit of 2^30", last_pos);
+    if (qdb_session_reserve(s, (int)last_pos + 1)) return -1;
+    return ensure_rope(s->m, (int)last_pos + 1);
 }
 
 // A paged session runs as a batch of one. Its final-normed hidden state is what
@@ -857,7 +862,7 @@ extern "C" int qdb_decode_greedy(qdb_session *s, int first_token, int pos, int n
     if (first_token < 0 || first_token >= m->cfg.vocab) return fail("token %d out of range", first_token);
     if (pos < 0) return fail("negative position");
     if (s->pool) return qdb_decode_greedy_batch(&s, 1, &first_token, &pos, n_steps, tokens_out);
-    if (set_dev(m) || prep_pos(s, pos + n_steps - 1)) return -1;
+    if (set_dev(m) || prep_pos(s, (long long)pos + n_steps - 1)) return -1;
     if (m->tok_cap < n_steps + 1) {
         cudaFree(m->tok_dev);
         m->tok_cap = 0;
@@ -1015,7 +1020,7 @@ static int paged_call(qdb_model *m, qdb_session *const *ss, int n, const int *le
 
 // Room for position last[i] (-1: none) of every session of a call. Where a pool
 // runs out, the pages this call has taken go back.
-static int reserve_all(qdb_session *const *ss, int n, const std::vector<int> &last) {
+static int reserve_all(qdb_session *const *ss, int n, const std::vector<long long> &last) {
     std::vector<size_t> had(n);
     for (int i = 0; i < n; i++) {
         had[i] = ss[i]->pages.size();
@@ -1220,9 +1225,9 @@ static int prefill_rows(qdb_session *const *ss, int nsess, const int *lens, cons
     const int T = (int)total;
     if (set_dev(m)) return -1;
     if (paged_kind(ss, nsess) < 0) return -1;
-    std::vector<int> last(nsess, -1);
+    std::vector<long long> last(nsess, -1);
     for (int i = 0; i < nsess; i++)
-        if (lens[i]) last[i] = starts[i] + lens[i] - 1;
+        if (lens[i]) last[i] = (long long)starts[i] + lens[i] - 1;
     if (reserve_all(ss, nsess, last)) return -1;
     if (ensure_rows(m, T, false)) return -1;
     RowScratch &r = m->rs;
@@ -1330,8 +1335,8 @@ static int batch_setup(qdb_session *const *ss, int n, const int *pos, int extra_
     if (kind && !pc) return fail("this call does not take paged sessions");
     if (set_dev(m) || ensure_rows(m, n, true)) return -1;
     std::vector<QdbRowKV> rk(n);
-    std::vector<int> last(n);
-    for (int b = 0; b < n; b++) last[b] = pos[b] + extra_steps;
+    std::vector<long long> last(n);
+    for (int b = 0; b < n; b++) last[b] = (long long)pos[b] + extra_steps;
     if (reserve_all(ss, n, last)) return -1;
     for (int b = 0; b < n; b++) rk[b] = QdbRowKV{ss[b]->kc, ss[b]->vc, ss[b]->cap, pos[b]};
     if (max_pos) {

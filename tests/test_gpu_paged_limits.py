@@ -58,3 +58,49 @@ def test_append_leaves_out_rows_behind_the_table(pkg, dtype, layout, rope, over,
         assert torch.equal(c.view(torch.int16), c0.view(torch.int16))
     err = pool.err.tolist()
     assert err[:2] == [3, 2] and err[2] in (0, 1) and err[3] in pos[pos >= full]
+
+
+# ---------------------------------------------------------------- positions behind what an int holds
+@pytest.fixture(scope="module")
+def world(pkg, synth):
+    ws = synth.WeightSet(synth.PRESETS["small"], seed=0, norm_jitter=0.1)
+    return ws, pkg.Model(ws, device=0, mask_eos=True)
+
+
+@pytest.mark.parametrize("paged", [False, True])
+def test_positions_behind_the_limit_are_refused(pkg, synth, world, paged):
+    """Positions whose sum with the steps or rows passes 2^30 or 31 bits: refused before any launch,
+    the session's capacity as it was, and the session still of use."""
+    ws, model = world
+    pool = pkg.PagePool(model, 16, 16)
+    make = (lambda: pool.session(32)) if paged else (lambda: model.session(256))
+    s, t = make(), make()
+    cap, free = s.capacity, pool.free_pages
+    emb = synth.prompt_embeddings(ws, synth.audio_embeddings(ws.cfg, 30, seed=2))[:30]
+    top = (1 << 31) - 1
+    limit = "limit of 2\\^30"
+    for pos in (1 << 30, top - 9, top - 1, top):
+        for steps in (1, 8, 10, 200):
+            with pytest.raises(pkg.QdbError, match=limit):
+                s.decode_greedy(3, pos, steps)
+            with pytest.raises(pkg.QdbError, match=limit):
+                pkg.decode_greedy_batch([s, t], [3, 4], [pos, 0], steps)
+            with pytest.raises(pkg.QdbError, match=limit):
+                pkg.decode_sample_batch([t, s], [3, 4], [0, pos], np.full((steps, 2), 0.5))
+        with pytest.raises(pkg.QdbError, match=limit):
+            s.forward(emb[0], pos)
+        with pytest.raises(pkg.QdbError, match=limit):
+            pkg.forward_batch([s, t], emb[:2], [pos, 0])
+        with pytest.raises(pkg.QdbError, match=limit):
+            s.prefill(emb, pos)
+        with pytest.raises(pkg.QdbError, match=limit):
+            pkg.prefill_batch([t, s], [emb[:3], emb], [0, pos])
+    with pytest.raises(pkg.QdbError, match=limit):
+        s.decode_greedy(3, (1 << 30) - 4, 5)
+    with pytest.raises(pkg.QdbError, match=limit):
+        s.prefill(emb, (1 << 30) - 29)
+    for n in ((1 << 30) + 1, top):
+        assert pkg.lib.qdb_session_reserve(s.h, n) == -1
+    assert (s.capacity, pool.free_pages) == (cap, free)
+    s.prefill(emb, 0)
+    assert s.forward(emb[3], 30)[0] >= 0
