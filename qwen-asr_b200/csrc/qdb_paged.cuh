@@ -145,15 +145,26 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, unsigned parity) {
                  : "memory");
     return ok != 0;
 }
-// Bounded wait; false = ran out (recorded).
-__device__ __forceinline__ bool bar_wait(uint32_t bar, unsigned parity, int *err) {
-    if (bar_try(bar, parity)) return true;
+// (without waiting; bar_try may sleep until the phase ends)
+__device__ __forceinline__ bool bar_test(uint32_t bar, unsigned parity) {
+    uint32_t ok;
+    asm volatile("{ .reg .pred p; mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+                 : "=r"(ok)
+                 : "r"(bar), "r"(parity)
+                 : "memory");
+    return ok != 0;
+}
+// Bounded wait; false = ran out (recorded). The waits that drain a CTA's own
+// copies or products before it exits take the fixed limit.
+__device__ __forceinline__ bool bar_wait(uint32_t bar, unsigned parity, int *err, long long limit = QDB_SPIN_LIMIT_CYCLES) {
+    if (bar_test(bar, parity)) return true;
     const long long t0 = clock64();
-    while (!bar_try(bar, parity))
-        if (clock64() - t0 > QDB_SPIN_LIMIT_CYCLES) {
+    do {
+        if (clock64() - t0 >= limit) {
             set_error(err, QDB_ERR_BARRIER_TIMEOUT);
             return false;
         }
+    } while (!bar_try(bar, parity));
     return true;
 }
 __device__ __forceinline__ void fence_bar_init() {
@@ -240,6 +251,8 @@ struct QdbDecodeScratch {
     int ctas;
 };
 cudaError_t qdb_decode_scratch_alloc(int device, QdbDecodeScratch *s);  // on the current device
+// Limit of the kernel's data waits in cycles, on the current device.
+extern "C" cudaError_t qdb_set_wait_limit_paged_decode(long long cycles);
 cudaError_t qdb_launch_paged_decode(const QdbPagedAttnArgs &a, int type, const QdbDecodeScratch &ws, cudaStream_t st);
 cudaError_t qdb_launch_paged_prompt(const QdbPagedAttnArgs &a, int type, cudaStream_t st);
 

@@ -371,7 +371,7 @@ __global__ void __launch_bounds__(DW * 32, 1)
             }
         }
         const int s = i % NS;
-        alive = bar_wait(full0 + 8 * s, (i / NS) & 1, a.bt.err);
+        alive = bar_wait(full0 + 8 * s, (i / NS) & 1, a.bt.err, qdb_wait_limit_c);
         if (__any_sync(0xffffffffu, !alive)) {
             alive = false;
             break;
@@ -597,6 +597,8 @@ cudaError_t launch(const CUtensorMap &mk, const CUtensorMap &mv, const QdbPagedA
 }
 
 }  // namespace
+
+QDB_WAIT_LIMIT_SETTER(qdb_set_wait_limit_paged_decode)
 
 cudaError_t qdb_launch_paged_decode(const QdbPagedAttnArgs &a, int type, const QdbDecodeScratch &ws, cudaStream_t st) {
     CUtensorMap mk, mv;

@@ -565,6 +565,7 @@ extern "C" int qdb_model_set_wait_limit(qdb_model *m, long long cycles) {
     CK(qdb_step_kernel_w7()->set_wait_limit(cycles));
     CK(qdb_set_wait_limit_tcgemm(cycles));
     CK(qdb_set_wait_limit_bstep(cycles));
+    CK(qdb_set_wait_limit_paged_decode(cycles));
     return 0;
 }
 

@@ -1,0 +1,72 @@
+"""GPU: waits of the paged kernels that run out.
+
+With the limit at 0 cycles a wait gives up at its first unsuccessful check: the kernel records it
+in the error words, lets its own copies land and returns. (A single short history may find every
+tile there already; its output is right then.) With the limit restored the next call is right.
+"""
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from test_gpu_paged import Pool, check_attention, queries, run_decode, stream  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def world(pkg, synth):
+    ws = synth.WeightSet(synth.PRESETS["tiny"], seed=12, norm_jitter=0.1)
+    return ws, synth.audio_embeddings(ws.cfg, 40, seed=4), pkg.Model(ws, device=0, mask_eos=True)
+
+
+class limit:
+    """The data waits' limit, in cycles, inside a with block."""
+
+    def __init__(self, model, cycles):
+        self.model, self.cycles = model, cycles
+
+    def __enter__(self):
+        torch.cuda.synchronize()
+        self.model.set_wait_limit(self.cycles)
+
+    def __exit__(self, *_):
+        torch.cuda.synchronize()
+        self.model.set_wait_limit(-1)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("heads,lens", [(4, [404]), (16, [700, 0, 33, 5000]), (32, [20000, 17] + [300] * 40)])
+def test_decode_wait_runs_out(pkg, world, dtype, heads, lens):
+    model = world[2]
+    pool = Pool(pkg, lens, 2, 16, dtype, seed=heads)
+    q = queries(len(lens), heads, dtype)
+    for _ in range(3):
+        with limit(model, 0):
+            out = run_decode(pkg, pkg.PagedWorkspace(), pool, q)
+        if pool.err.tolist()[0] == 0 and len(lens) == 1:
+            check_attention(pool, q, out, [1])
+        else:
+            assert pool.err.tolist()[0] == 1
+        pool.err.zero_()
+        check_attention(pool, q, run_decode(pkg, pkg.PagedWorkspace(), pool, q), [1] * len(lens))
+
+
+def test_paged_session_recovers(pkg, world):
+    """Through the model: the step fails with the wait named, and the next one is right (the joins'
+    counters start again from zero)."""
+    ws, emb, model = world
+    pool = pkg.PagePool(model, 64, 16)
+    a, b, one = pool.session(400), pool.session(), model.session(64)
+    for s in (a, b, one):
+        s.prefill(emb[:20], 0)
+    x = np.stack([emb[20]] * 2)
+    _, want = pkg.forward_batch([one, one], x, [20, 20], want_logits=True)
+    for _ in range(3):
+        with limit(model, 0):
+            with pytest.raises(pkg.QdbError, match="bounded wait"):
+                pkg.forward_batch([a, b], x, [20, 20])
+            with pytest.raises(pkg.QdbError, match="bounded wait"):
+                pkg.decode_greedy_batch([a, b], [3, 4], [20, 20], 6)
+        _, got = pkg.forward_batch([a, b], x, [20, 20], want_logits=True)
+        assert np.abs(got - want).max() <= 2e-2
