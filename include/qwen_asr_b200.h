@@ -224,8 +224,9 @@ int qdb_forward_noalloc(qdb_session *s, const float *embed_dev, int pos, int *to
  * out" and the model stays usable. It applies to the waits of the persistent
  * decode step (one CTA waiting for another CTA's results or for its weight
  * copies), of the tensor-core GEMMs (a stage's copies, a free stage) and of
- * the one-token attention over pages (a tile's copies); the waits that drain a
- * CTA's own copies or MMAs before it exits keep the fixed one-second bound. The setting is per device (every model on the device of
+ * the attentions over pages (a tile's copies; in the prompt attention every wait
+ * of one role for another); the waits that drain a CTA's own copies or MMAs
+ * before it exits keep the fixed one-second bound. The setting is per device (every model on the device of
  * m), so it exists for tests of the error path and for callers that want a
  * stuck step reported sooner. cycles = 0 makes a wait give up at its first
  * unsuccessful check.

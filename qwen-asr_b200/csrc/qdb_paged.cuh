@@ -251,8 +251,9 @@ struct QdbDecodeScratch {
     int ctas;
 };
 cudaError_t qdb_decode_scratch_alloc(int device, QdbDecodeScratch *s);  // on the current device
-// Limit of the kernel's data waits in cycles, on the current device.
+// Limit of the kernels' data waits in cycles, on the current device.
 extern "C" cudaError_t qdb_set_wait_limit_paged_decode(long long cycles);
+extern "C" cudaError_t qdb_set_wait_limit_paged_prompt(long long cycles);  // (at most 3e9)
 cudaError_t qdb_launch_paged_decode(const QdbPagedAttnArgs &a, int type, const QdbDecodeScratch &ws, cudaStream_t st);
 cudaError_t qdb_launch_paged_prompt(const QdbPagedAttnArgs &a, int type, cudaStream_t st);
 

@@ -179,16 +179,21 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
+// Limit of the data waits in 32-bit cycles (well below where the counter comes
+// round; qdb_set_wait_limit_paged_prompt).
+__constant__ unsigned prompt_wait_limit = (unsigned)QDB_SPIN_LIMIT_CYCLES;
+
 // Bounded wait that also ends when another role has given up. (Short: it is
 // inlined at every wait. The error is recorded once, at the end.)
 __device__ __forceinline__ bool wait_on(PromptSmem &sm, uint32_t bar, unsigned parity) {
-    if (bar_try(bar, parity)) return true;
+    if (bar_test(bar, parity)) return true;
     const unsigned t0 = (unsigned)clock();
-    while (!bar_try(bar, parity))
-        if (*reinterpret_cast<volatile int *>(&sm.abort) || (unsigned)clock() - t0 > (unsigned)QDB_SPIN_LIMIT_CYCLES) {
+    do {
+        if (*reinterpret_cast<volatile int *>(&sm.abort) || (unsigned)clock() - t0 >= prompt_wait_limit) {
             *reinterpret_cast<volatile int *>(&sm.abort) = 1;
             return false;
         }
+    } while (!bar_try(bar, parity));
     return true;
 }
 
@@ -509,6 +514,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
             n_s += nt;
             item_done();
         }
+        tm_st_wait();  // (where a wait ran out: before the columns are given back)
     } else if (warp < 10) {
         // ------------------------------------------------ products: warp 8 the scores, warp 9 the outputs
         // (the whole warp runs this together, with values that are the same in all
@@ -735,22 +741,22 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                 item_done();
             }
         }
-        if (!ok) {  // given up: what is in flight lands first
-            const int ring_tiles = min(n_tile, (unsigned)S);
+        // what is in flight lands before the CTA ends, whatever role has given up
+        // (none has: its copies have been waited for, and these checks find them there)
+        const int ring_tiles = min(n_tile, (unsigned)S);
 #pragma unroll 1
-            for (int k = -2; k < ring_tiles; k++) {
-                uint32_t bar = smem_u32(&sm.stolen_bar);
-                unsigned parity = answered & 1;
-                if (k == -2 && asked == answered) continue;
-                if (k == -1) {
-                    if (!n_q) continue;
-                    bar = smem_u32(&sm.q_full), parity = (n_q - 1) & 1;
-                } else if (k >= 0) {  // (the ring's tiles, the newest first)
-                    if (st-- == 0) st = S - 1, phase ^= 1;
-                    bar = smem_u32(&full[st]), parity = phase;
-                }
-                bar_wait(bar, parity, err);
+        for (int k = -2; k < ring_tiles; k++) {
+            uint32_t bar = smem_u32(&sm.stolen_bar);
+            unsigned parity = answered & 1;
+            if (k == -2 && asked == answered) continue;
+            if (k == -1) {
+                if (!n_q) continue;
+                bar = smem_u32(&sm.q_full), parity = (n_q - 1) & 1;
+            } else if (k >= 0) {  // (the ring's tiles, the newest first)
+                if (st-- == 0) st = S - 1, phase ^= 1;
+                bar = smem_u32(&full[st]), parity = phase;
             }
+            bar_wait(bar, parity, err);
         }
         __syncwarp();
     }
@@ -782,6 +788,11 @@ cudaError_t launch(const CUtensorMap &mq, const CUtensorMap &mk, const CUtensorM
 }
 
 }  // namespace
+
+extern "C" cudaError_t qdb_set_wait_limit_paged_prompt(long long cycles) {
+    const unsigned c = (unsigned)(cycles < 3000000000ll ? cycles : 3000000000ll);
+    return cudaMemcpyToSymbol(prompt_wait_limit, &c, sizeof(c));
+}
 
 cudaError_t qdb_launch_paged_prompt(const QdbPagedAttnArgs &a, int type, cudaStream_t st) {
     CUtensorMap mq, mk, mv;

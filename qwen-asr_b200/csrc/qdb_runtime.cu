@@ -566,6 +566,7 @@ extern "C" int qdb_model_set_wait_limit(qdb_model *m, long long cycles) {
     CK(qdb_set_wait_limit_tcgemm(cycles));
     CK(qdb_set_wait_limit_bstep(cycles));
     CK(qdb_set_wait_limit_paged_decode(cycles));
+    CK(qdb_set_wait_limit_paged_prompt(cycles));
     return 0;
 }
 

@@ -9,7 +9,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from test_gpu_paged import Pool, check_attention, queries, run_decode, stream  # noqa: E402
+from test_gpu_paged import Pool, check_attention, queries, run_decode, run_prompt  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -69,4 +69,54 @@ def test_paged_session_recovers(pkg, world):
             with pytest.raises(pkg.QdbError, match="bounded wait"):
                 pkg.decode_greedy_batch([a, b], [3, 4], [20, 20], 6)
         _, got = pkg.forward_batch([a, b], x, [20, 20], want_logits=True)
+        assert np.abs(got - want).max() <= 2e-2
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("heads,kv_heads,lens,q_lens", [
+    (4, 2, [1], [1]), (16, 8, [404], [404]), (4, 4, [900, 0, 3000], [900, 0, 5]), (16, 1, [300] * 40, [70] * 40),
+    (8, 4, [40] * 300, [13] * 300), (16, 8, [9000, 4000], [3000, 4000])], ids=str)
+def test_prompt_wait_runs_out(pkg, world, dtype, heads, kv_heads, lens, q_lens):
+    model = world[2]
+    pool = Pool(pkg, lens, kv_heads, 32, dtype, seed=heads)
+    q = queries(sum(q_lens), heads, dtype)
+    for _ in range(3):
+        with limit(model, 0):
+            run_prompt(pkg, pool, q, q_lens)
+        assert pool.err.tolist()[0] == 1
+        pool.err.zero_()
+        check_attention(pool, q, run_prompt(pkg, pool, q, q_lens), q_lens)
+
+
+@pytest.mark.parametrize("cycles", [1, 300, 1000, 3000, 10000, 30000])
+def test_prompt_gives_up_anywhere(pkg, world, cycles):
+    """Limits between the shortest and the longest wait: roles give up at different places, some
+    after their last copy; either the error is recorded or the output is right."""
+    model = world[2]
+    lens, q_lens = [700, 1, 90, 4000, 129], [700, 1, 33, 300, 129]
+    pool = Pool(pkg, lens, 2, 16, "bf16", seed=cycles)
+    q = queries(sum(q_lens), 8, "bf16")
+    for _ in range(5):
+        with limit(model, cycles):
+            out = run_prompt(pkg, pool, q, q_lens)
+        if pool.err.tolist()[0] == 0:
+            check_attention(pool, q, out, q_lens)
+        else:
+            assert pool.err.tolist()[0] == 1
+        pool.err.zero_()
+        check_attention(pool, q, run_prompt(pkg, pool, q, q_lens), q_lens)
+
+
+def test_paged_prefill_recovers(pkg, world):
+    ws, emb, model = world
+    pool = pkg.PagePool(model, 64, 16)
+    a, one = pool.session(), model.session(64)
+    one.prefill(emb[:30], 0)
+    _, _, want = one.forward(emb[30], 30, want_logits=True)
+    for _ in range(3):
+        with limit(model, 0):
+            with pytest.raises(pkg.QdbError, match="bounded wait"):
+                a.prefill(emb[:30], 0)
+        a.prefill(emb[:30], 0)
+        _, _, got = a.forward(emb[30], 30, want_logits=True)
         assert np.abs(got - want).max() <= 2e-2
