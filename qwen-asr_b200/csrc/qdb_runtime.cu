@@ -1189,14 +1189,15 @@ static int run_rows(qdb_model *m, int n, const PrefillPlan *pf, const QdbRowKV *
     return 0;
 }
 
-// Reads (and clears) the tensor-core GEMMs' device error words after a sync.
+// Reads (and clears) the tensor-core GEMMs' device error words after a sync. Cleared
+// on the model's stream, which the legacy default stream's work is not ordered with.
 static int check_rows_err(qdb_model *m) {
     int ev[4] = {0, 0, 0, 0};
     CK(cudaMemcpy(ev, m->rs.err, sizeof(ev), cudaMemcpyDeviceToHost));
     if (ev[0]) {
-        cudaMemset(m->rs.err, 0, sizeof(ev));
+        CK(cudaMemsetAsync(m->rs.err, 0, sizeof(ev), m->st));
         // (a part that never came leaves a counter of the joins behind)
-        if (m->rs.pdec.cnt) cudaMemset(m->rs.pdec.cnt, 0, sizeof(unsigned) * m->rs.pdec.ctas);
+        if (m->rs.pdec.cnt) CK(cudaMemsetAsync(m->rs.pdec.cnt, 0, sizeof(unsigned) * m->rs.pdec.ctas, m->st));
         return fail("device error code %d in a tensor-core GEMM (%s)", ev[0],
                     ev[0] == QDB_ERR_BOUNDS ? "an access refused by a bounds check" : "a bounded wait ran out");
     }

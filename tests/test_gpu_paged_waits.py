@@ -120,3 +120,22 @@ def test_paged_prefill_recovers(pkg, world):
         a.prefill(emb[:30], 0)
         _, _, got = a.forward(emb[30], 30, want_logits=True)
         assert np.abs(got - want).max() <= 2e-2
+
+
+def test_failed_steps_followed_at_once(pkg, world):
+    """The error words and the joins' counters are cleared ahead of the call that follows."""
+    ws, emb, model = world
+    pool = pkg.PagePool(model, 128, 16)
+    a, one = pool.session(1500), model.session(64)
+    for s in (a, one):
+        s.prefill(emb[:20], 0)
+    _, _, want = one.forward(emb[20], 20, want_logits=True)
+    for _ in range(100):
+        model.set_wait_limit(0)
+        try:
+            with pytest.raises(pkg.QdbError, match="bounded wait"):
+                a.forward(emb[20], 1200)
+        finally:
+            model.set_wait_limit(-1)
+        _, _, got = a.forward(emb[20], 20, want_logits=True)
+        assert np.abs(got - want).max() <= 2e-2
