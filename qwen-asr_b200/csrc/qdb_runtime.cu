@@ -1189,7 +1189,7 @@ static int run_rows(qdb_model *m, int n, const PrefillPlan *pf, const QdbRowKV *
     return 0;
 }
 
-// Reads (and clears) the tensor-core GEMMs' device error words after a sync. Cleared
+// Reads (and clears) the row kernels' device error words after a sync. Cleared
 // on the model's stream, which the legacy default stream's work is not ordered with.
 static int check_rows_err(qdb_model *m) {
     int ev[4] = {0, 0, 0, 0};
@@ -1198,8 +1198,10 @@ static int check_rows_err(qdb_model *m) {
         CK(cudaMemsetAsync(m->rs.err, 0, sizeof(ev), m->st));
         // (a part that never came leaves a counter of the joins behind)
         if (m->rs.pdec.cnt) CK(cudaMemsetAsync(m->rs.pdec.cnt, 0, sizeof(unsigned) * m->rs.pdec.ctas, m->st));
-        return fail("device error code %d in a tensor-core GEMM (%s)", ev[0],
-                    ev[0] == QDB_ERR_BOUNDS ? "an access refused by a bounds check" : "a bounded wait ran out");
+        if (ev[0] == QDB_ERR_BOUNDS)
+            return fail("device error code %d in the row kernels (an access refused by a bounds check; check %d: %d %d)",
+                        ev[0], ev[1], ev[2], ev[3]);
+        return fail("device error code %d in the row kernels (a bounded wait ran out)", ev[0]);
     }
     return 0;
 }

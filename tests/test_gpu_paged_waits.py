@@ -139,3 +139,12 @@ def test_failed_steps_followed_at_once(pkg, world):
             model.set_wait_limit(-1)
         _, _, got = a.forward(emb[20], 20, want_logits=True)
         assert np.abs(got - want).max() <= 2e-2
+
+
+def test_error_names_the_row_kernels(pkg, world):
+    """The words are shared by the GEMMs and the attention kernels: the message does not single one out."""
+    ws, emb, model = world
+    s = pkg.PagePool(model, 64, 16).session()
+    with limit(model, 0):
+        with pytest.raises(pkg.QdbError, match=r"in the row kernels \(a bounded wait ran out\)"):
+            s.prefill(emb[:30], 0)
