@@ -30,7 +30,8 @@ step streams them from HBM; no flush is needed.
 from the reference sources) on this host for the same config: the decode of
 one utterance (the reference decodes utterances one after another), sampled
 evenly over the whole decode context range of the config at every step. This
-arm never loads the CUDA library.
+arm never loads the CUDA library. Where oracle/_ref is not built it prints
+{"impl": "reference", "unavailable": ...}.
 """
 from __future__ import annotations
 
@@ -1048,6 +1049,12 @@ def main():
     if args.profile_step:
         profile_step(args)
     elif args.impl == "reference":
+        from oracle.pyoracle import ref_so_path
+        if not ref_so_path():  # (never the restatement under the reference's name)
+            if dist_env()[1] == 0:
+                print(json.dumps({"impl": "reference", "unavailable": "oracle/_ref is not built: the reference's "
+                                                                      "sources are not on this machine"}))
+            return
         run_streams_reference(args) if args.config == "c4" else run_reference(args)
     else:
         run_streams_ours(args) if args.config == "c4" else run_ours(args)
