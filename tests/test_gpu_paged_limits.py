@@ -4,7 +4,8 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from test_gpu_paged import D, T, Pool, append64, half_step, rope_table, starts_of, stream  # noqa: E402
+from test_gpu_paged import (D, T, Pool, append64, half_step, queries, rope_table, run_decode, starts_of,  # noqa: E402
+                            stream)
 
 pytestmark = pytest.mark.gpu
 
@@ -104,3 +105,33 @@ def test_positions_behind_the_limit_are_refused(pkg, synth, world, paged):
     assert (s.capacity, pool.free_pages) == (cap, free)
     s.prefill(emb, 0)
     assert s.forward(emb[3], 30)[0] >= 0
+
+
+# ---------------------------------------------------------------- values that are not finite
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("heads,n", [(4, 300), (32, 300), (4, 20)])
+@pytest.mark.parametrize("scale", [0.0, 1e-3])
+def test_decode_infinite_values(pkg, dtype, heads, n, scale):
+    """An infinite V gives an infinite output of its sign to the heads that see it, NaN gives NaN,
+    and the other dims and heads stay as they were (f16: a weight below its smallest value, 2^-32 of
+    the largest, gives NaN)."""
+    ws = pkg.PagedWorkspace()
+    pool = Pool(pkg, [n, n], 2, 16, dtype, seed=n)
+    q = queries(2, heads, dtype)
+    clean = run_decode(pkg, ws, pool, q, scale=scale)
+    inf = float("inf")
+    for key, dim, x in ((0, 3, inf), (n - 1, 127, -inf), (n // 2, 9, float("nan"))):
+        pg, sl = pool.where(0, n)
+        pool.v[pg[key], 1, sl[key], dim] = x
+    out = run_decode(pkg, ws, pool, q, scale=scale)
+    g = heads // 2
+    assert torch.equal(out[1], clean[1]) and torch.equal(out[0, :g], clean[0, :g])
+    bad = out[0, g:]
+    k = pool.get(0, n)[0][:, 1].double()
+    p = torch.softmax((q[0, g:].double() @ k.T) * (scale or 128 ** -0.5), -1)
+    least = (2.0 ** -31 if dtype == "f16" else 0.0) * p.max(-1)[0]
+    for key, dim, x in ((0, 3, inf), (n - 1, 127, -inf)):
+        assert ((bad[:, dim] == x) | (torch.isnan(bad[:, dim]) & (p[:, key] <= least))).all()
+    assert torch.isnan(bad[:, 9]).all()
+    rest = [d for d in range(128) if d not in (3, 9, 127)]
+    assert torch.equal(bad[:, rest], clean[0, g:][:, rest])
