@@ -106,7 +106,9 @@ int qdb_session_reserve(qdb_session *s, int positions);
  * and qdb_decode_sample_batch, not in qdb_trace_step, qdb_trace_batch_step and
  * qdb_forward_noalloc; the sessions of one call share one pool. qdb_forward and
  * qdb_decode_greedy run them as a batch of one (hidden_out then carries 16
- * mantissa bits). Freeing a pool detaches its sessions: their calls fail, and
+ * mantissa bits). Their attention reads each query in one fp16, the type of the
+ * cached keys; contiguous sessions carry queries as an fp16 pair of about 22
+ * bits. Freeing a pool detaches its sessions: their calls fail, and
  * they are still to be freed. */
 typedef struct qdb_pool qdb_pool;
 qdb_pool *qdb_pool_create(qdb_model *m, int n_pages, int page_size);
@@ -489,8 +491,9 @@ typedef struct {
  * the weights before it sum to less than top_p of the top_k's, and w_i >=
  * min_p (the first token always stays). The result is the first token that
  * stays, in index order, at which the running sum of the weights exceeds
- * uniform * total. Sums are exact integers in units of 2^-45 of the largest
- * weight: the result does not depend on the run. NaN and -inf logits are never
+ * uniform * total. Weights are computed to 2^-42 of each and rounded to 2^-45 of
+ * the largest; their sums are exact integers, so that the result does not depend
+ * on the run. NaN and -inf logits are never
  * drawn; a row with nothing else gives -1. */
 int qdb_sample(const void *logits, int type, long long row_stride, int rows, int vocab, const qdb_sampling *s,
                int *tokens_out, void *stream);

@@ -66,7 +66,8 @@ struct Raw8<SrcF32> {
 // only, 77 us (6.1 TB/s, 95 % of the copy) with four vectors, 87 with two, 96 with
 // one (bound by the look-ups' instructions), 88 with eight; 3721 rows, f32 to f16,
 // norms and rotation, 17.8 us (5.2 TB/s) with two, 25 with one, 21 with four; 64
-// rows 4.4 us, which is the launch and the look-ups. Six CTAs per SM: 80 registers.
+// rows 4.4 us, which is the launch and the look-ups. Six CTAs per SM: 80 registers
+// (of the 16-bit sources' four vectors 20 to 32 bytes spill).
 constexpr int AP_THREADS = 128, AP_GROUPS = AP_THREADS / 8, AP_CTAS = 6;
 template <typename S>
 constexpr int ap_vecs = 4;

@@ -10,7 +10,10 @@
 // pair are computed together, 16 keys at a time, with a running maximum m and
 // sum l per head in f32:
 //   S^T = K q^T      (keys x heads: K as the row operand, ldmatrix)
-//   P = 2^(S c - m)  (c = scale log2 e), rounded to the cache's type
+//   P = 2^(S c - m)  (c = scale log2 e), rounded to the cache's type (error against
+//                     64 bits 1.25 times that of f32 arithmetic; as a pair of the
+//                     type 1.00 times, but one short history 8.6 -> 8.8 us, 64 of
+//                     them 30.6 -> 31.4)
 //   O^T += V^T P^T   (dims x heads: V as the row operand, transposed ldmatrix;
 //                     P^T by movmatrix from the S^T fragment)
 // A pair that lies in several warps' ranges leaves partial (m, l, O); the
@@ -19,9 +22,9 @@
 // does not depend on timing.
 //
 // Measured (L2 cold): 256 ragged sequences of 1 to 1500 tokens, 16 heads on 8
-// key heads, bf16, 144 us, and 8 of 24000 to 32768, 32 heads on 4, 78 us: 91 %
-// and 88 % of the copy bandwidth for their K and V bytes. 64 sequences of 404
-// to 660, f16, 31 us against 21 for the bytes; one of 404 8.1 us against 0.3:
+// key heads, bf16, 146 us, and 8 of 24000 to 32768, 32 heads on 4, 81 us: 90 %
+// and 85 % of the copy bandwidth for their K and V bytes. 64 sequences of 404
+// to 660, f16, 31 us against 21 for the bytes; one of 404 8.6 us against 0.3:
 // the fixed chain of launch, lengths, page numbers, first tiles and the join
 // over CTAs. A first version, one warp per (row, query head) with scalar
 // products, took 734 us for the 256, 11.5 ms, 344 and 91 us.
@@ -38,12 +41,13 @@ constexpr int DW = 8;             // warps per CTA
 constexpr int TILE = 16;          // keys per tile (a page holds whole tiles)
 constexpr int TILE_B = 4096;      // bytes of a tile's K (or V)
 constexpr int MAX_G = 16;         // query heads per key head
-// Tiles of a CTA, on average, below which a pair is not cut further. 404 keys
-// of 8 key heads: 9.5 us at 4, 9.9 at 8, 11.6 at 16 (before later steps); 4000 keys: 11.8 us at 4 to
-// 16, 13.8 at 32.
+// Tiles of a CTA, on average, below which a pair is not cut further. One sequence of
+// 200 keys of 8 key heads: 8.1 us at 2 and 4, 9.5 at 8; four of 404: 8.8 at 2 and 4,
+// 9.6 at 8; one of 1000 or 4000: the same at all three.
 constexpr int MIN_TILES = 4;
 // Tiles of a CTA from which the pairs' borders do not matter: 8 sequences of 24000
-// to 32768 with 4 key heads 80.1 us on 128 CTAs, 78.2 on all 148.
+// to 32768 with 4 key heads 83 us on 128 CTAs, 80.8 on all 148; 20 of 20000 to 30000
+// with 2 97.5 on 120, 90.9 on all; one of 100000 with 8 73 and 71.8.
 constexpr int MANY_TILES = 128;
 constexpr float P_SHIFT = 8.0f;   // P is scaled by 2^8: f16 keeps weights down to 2^-32 of the largest
 

@@ -1604,7 +1604,9 @@ extern "C" int qdb_forward_batch(qdb_session *const *sessions, int n, const floa
     const int S = std::min(64, std::max(1, (maxp + 1 + 64 * QDB_AR_ITERS - 1) / (64 * QDB_AR_ITERS)));
     // the captured launches bake in the row count, the split count, every
     // scratch pointer, the RoPE table (reallocated when a session grows past
-    // it) and the EOS mask
+    // it) and the EOS mask. (A paged step bakes in the table's length too: a power of
+    // two no smaller than table_stride pages, so it holds every position that a
+    // replay of the same table_stride can reach.)
     auto graph_key = [&]() {
         return std::vector<const void *>{(const void *)(intptr_t)n, (const void *)(intptr_t)S,
                                          (const void *)(intptr_t)m->mask_eos, m->rope, r.X, r.XH, r.XL, r.QKV, r.Q,

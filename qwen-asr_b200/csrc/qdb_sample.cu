@@ -12,8 +12,10 @@
 //
 // Sums are 64-bit integers: w is rounded to a multiple of 2^-45 (a token more
 // than 31.5 T below the maximum is never drawn), so a sum over up to 2^18 tokens
-// is exact, independent of the order of the atomics, and a border between two
-// tokens is off by at most 2^-46 of the largest weight per token summed.
+// is exact and independent of the order of the atomics. The weights themselves
+// are off by up to 2^-42.6 of each (a polynomial cut after degree 5) and that
+// rounding, 2^-46 of the largest; a border between two tokens is off by the sum
+// of these.
 // (uniform = 0 asks for the first kept token of any weight above zero: there
 // every such token counts 1.)
 //
@@ -34,11 +36,14 @@
 // Measured, 151936 f32 logits a row: one row with top_k 50 and top_p 0.95 12.6 us
 // (4.7 us greedy, 40 us top_p alone), 64 rows of mixed parameters 49 us, 18 rows of
 // top_k 50 17 us. Reading the logits would take 0.1 and 6 us: what bounds it is
-// the chain of cluster barriers (1000 clocks each) and passes for one row, and the
-// instructions per token for many (45 in the pass that weighs and counts all
-// tokens: a weight to 2^-45 takes about 11 64-bit operations). A first version,
-// one CTA per row and the logits read again in every pass, took 609 and
-// 3176 us.
+// one row's own chain of passes and cluster barriers (1000 clocks each). Clocks of
+// a row with top_p alone, 73500 in all: start 2000, logits and maximum 6900, the
+// pass that weighs and counts all tokens 14200 (16 warps of an SM: its 45
+// instructions per token alone would be 6700), barrier and merge of the histograms
+// 5200, bins of the cut 5900, their keys 1600, the pass that weighs the tokens
+// above them 16900, sort and cut 9600, the sum below 5000, the draw 6200. A mixed
+// batch waits for such rows. A first version, one CTA per row and the logits read
+// again in every pass, took 609 and 3176 us. (40 bytes of the 64 registers spill.)
 #include <cooperative_groups.h>
 #include <math.h>
 #include <stdio.h>
@@ -996,8 +1001,9 @@ __global__ void __launch_bounds__(ST, 2) sample_kernel(const QdbSampleArgs a, in
 
 template <int TYPE>
 cudaError_t launch(const QdbSampleArgs &a, cudaStream_t st) {
-    // at least 16K tokens per CTA: below that the cluster's barriers cost more
-    // than the shorter passes save
+    // at least 16K tokens per CTA. 50257 tokens, top_k 50 / top_p alone: one row 11.5 /
+    // 28.4 us, 64 rows 16.4 / 45; with 8K 10.4 / 23.8 and 29.7 / 63 (the clusters no
+    // longer all run at once), with 32K 13.5 / 43 and 15.2 / 48
     int C = 1;
     while (C < SC && a.vocab > C * 16384) C <<= 1;
     const int slice = ((a.vocab + C - 1) / C + 31) & ~31;
