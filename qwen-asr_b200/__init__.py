@@ -728,9 +728,13 @@ def decode_sample_batch(sessions, first_tokens, pos, uniform, temperature=None, 
     """decode_greedy_batch with drawn tokens: uniform [n_steps, n] random numbers in
     [0, 1), parameters [n] (None = off). Returns the tokens [n_steps, n]."""
     n = len(sessions)
-    u = np.ascontiguousarray(uniform, dtype=np.float32).reshape(-1, n)
+    u = np.ascontiguousarray(uniform, dtype=np.float32)
     f = np.ascontiguousarray(first_tokens, dtype=np.int32)
     p = np.ascontiguousarray(pos, dtype=np.int32)
+    if f.size != n or p.size != n or u.size % max(n, 1) or u.ndim > 1 and u.shape[-1] != n:
+        raise QdbError(f"first tokens, positions and random numbers of shapes {f.shape}, {p.shape}, {u.shape} "
+                       f"for {n} sessions")
+    u = u.reshape(-1, n)
     par = [None if v is None else np.ascontiguousarray(np.broadcast_to(np.asarray(v, t), (n,)))
            for v, t in ((temperature, np.float32), (top_k, np.int32), (top_p, np.float32), (min_p, np.float32))]
     s = QdbSampling(*[None if v is None else v.ctypes.data for v in par], u.ctypes.data)

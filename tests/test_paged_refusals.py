@@ -149,3 +149,16 @@ def test_host_pointers_are_refused(pkg):
             op(kv(pkg, k=host, v=host), batch(pkg, kv_lens=host, tables=host), q=host, o=host)
     with pytest.raises(pkg.QdbError, match="not a device pointer" if has_gpu() else "CUDA"):
         pkg.sample(host, 1, 100, host, host)
+
+
+def test_sampled_loop_arrays_of_other_lengths(pkg):
+    """One first token, position and column of random numbers per session: nothing shorter is read
+    behind its end, nothing longer is cut."""
+    two = [type("S", (), {"h": None})()] * 2
+    for f, p, u, kw in (([1], [0, 0], [[0.5, 0.5]], {}), ([1, 2], [0], [[0.5, 0.5]], {}), ([1, 2, 3], [0, 0], [[0.5, 0.5]], {}),
+                        ([1, 2], [0, 0], [[0.5]], {}), ([1, 2], [0, 0], [[0.5] * 4], {}), ([1, 2], [0, 0], [0.5] * 3, {}),
+                        ([1, 2], [0, 0], [[0.5, 0.5]], dict(top_k=[1, 2, 3])), (1, [0, 0], [[0.5, 0.5]], {})):
+        with pytest.raises((pkg.QdbError, ValueError), match="shape|broadcast|sessions"):
+            pkg.decode_sample_batch(two, f, p, u, **kw)
+    with pytest.raises(pkg.QdbError, match="session"):  # (of the right lengths: the library's own check)
+        pkg.decode_sample_batch(two, [1, 2], [0, 0], [[0.5, 0.5]] * 3)
