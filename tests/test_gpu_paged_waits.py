@@ -1,8 +1,8 @@
 """GPU: waits of the paged kernels that run out.
 
 With the limit at 0 cycles a wait gives up at its first unsuccessful check: the kernel records it
-in the error words, lets its own copies land and returns. (A single short history may find every
-tile there already; its output is right then.) With the limit restored the next call is right.
+in the error words, lets its own copies land and returns. (Short histories may find every tile
+there already; their output is right then.) With the limit restored the next call is right.
 """
 import numpy as np
 import pytest
@@ -44,8 +44,8 @@ def test_decode_wait_runs_out(pkg, world, dtype, heads, lens):
     for _ in range(3):
         with limit(model, 0):
             out = run_decode(pkg, pkg.PagedWorkspace(), pool, q)
-        if pool.err.tolist()[0] == 0 and len(lens) == 1:
-            check_attention(pool, q, out, [1])
+        if pool.err.tolist()[0] == 0 and sum(lens) < 10000:  # (no more than a tile or two per warp)
+            check_attention(pool, q, out, [1] * len(lens))
         else:
             assert pool.err.tolist()[0] == 1
         pool.err.zero_()
